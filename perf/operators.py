@@ -23,7 +23,7 @@ own = False
 
 # coefficients of the quintic Newton-Schulz iteration
 NS = (3.4445, -4.7750, 2.0315)
-NORM_FLOOR = 1e-7
+NORM_FLOOR = 1e-30
 
 
 # ------------------------------------------------------------------- cases --

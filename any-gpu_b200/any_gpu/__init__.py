@@ -22,7 +22,8 @@ import numpy as np
 
 from . import _lib
 
-__all__ = ["GpuDevice", "GpuBuffer", "AnyGpuError", "PRECISIONS"]
+__all__ = ["GpuDevice", "GpuBuffer", "AnyGpuError", "PRECISIONS", "AdamW", "Muon", "QkNormRope",
+           "muon_tensors"]
 
 PRECISIONS = {"tf32": 0, "tf32x3": 1, "ffma": 2}
 _STATUS_NAMES = {0: "OK", 1: "SHAPE", 2: "INVALID", 3: "CUDA", 4: "OOM", 5: "NO_DEVICE",
@@ -79,6 +80,26 @@ class GpuBuffer:
 def _f32(data) -> np.ndarray:
     arr = np.ascontiguousarray(np.asarray(data, dtype=np.float32).reshape(-1))
     return arr
+
+
+def QkNormRope(batch: int, seq: int, q_heads: int, k_heads: int, dim: int, rot_dim=None,
+               eps: float = 1e-6, base: float = 10000.0, q_in=None, k_in=None, q_out=None,
+               k_out=None) -> "_lib.QkNormRopeShape":
+    """Geometry of `launch_qk_norm_rope` and its backward (agpu_qk_norm_rope).
+    Layouts are (seq_stride, head_stride, batch_stride) in elements; None =
+    contiguous [batch, seq, heads, dim].  rot_dim None = the whole head."""
+    def lay(st, heads):
+        return _lib.AttnLayout(*(st or (heads * dim, dim, seq * heads * dim)))
+    return _lib.QkNormRopeShape(batch, seq, q_heads, k_heads, dim,
+                                dim if rot_dim is None else rot_dim, eps, base,
+                                lay(q_in, q_heads), lay(k_in, k_heads), lay(q_out, q_heads),
+                                lay(k_out, k_heads))
+
+
+def muon_tensors(tensors):
+    """The host array `launch_muon` takes, from (param_ptr, grad_ptr,
+    momentum_ptr, rows, cols) tuples; a program builds it once and keeps it."""
+    return (_lib.MuonTensor * len(tensors))(*[_lib.MuonTensor(*t) for t in tensors])
 
 
 class GpuDevice:
@@ -175,6 +196,19 @@ class GpuDevice:
                                        C.byref(out)))
         # the H2D copy is stream-ordered from pageable memory: it has completed
         # (or been staged) before agpu_upload returns, so `arr` may be dropped.
+        return GpuBuffer(out.value, self)
+
+    def upload_i32(self, data) -> GpuBuffer:
+        """int32 values (token ids, positions) in a buffer of their own kind."""
+        arr = np.asarray(data)
+        if arr.size and arr.dtype.kind not in "iu":
+            raise TypeError(f"upload_i32: expected integers, got {arr.dtype}")
+        if arr.size and (arr.min() < -2**31 or arr.max() >= 2**31):
+            raise OverflowError("upload_i32: a value does not fit in 32 bits")
+        arr = np.ascontiguousarray(arr.reshape(-1), dtype=np.int32)
+        out = C.c_void_p()
+        _check(_lib.load().agpu_upload_i32(self._h, arr.ctypes.data_as(C.c_void_p), arr.size,
+                                           C.byref(out)))
         return GpuBuffer(out.value, self)
 
     def alloc(self, n: int) -> GpuBuffer:
@@ -385,6 +419,93 @@ class GpuDevice:
         _check(_lib.load().agpu_launch_swish_mul(self._h, g_ptr, u_ptr, o_ptr, rows, cols,
                                                  g_stride, u_stride, o_stride, stream or None))
 
+    # ------------------------------------------- ops for training on tokens --
+    def embedding(self, table, ids, tokens: int, vocab: int, dim: int,
+                  scale: float = 1.0) -> GpuBuffer:
+        """out[t] = scale * table[ids[t]] (agpu_embedding); ids from upload_i32,
+        -1 = padding (a zero row)."""
+        return self._new(_lib.load().agpu_embedding, table.handle, ids.handle, tokens, vocab, dim,
+                         C.c_float(scale))
+
+    def embedding_backward(self, grad_out, ids, tokens: int, vocab: int, dim: int,
+                           scale: float = 1.0) -> GpuBuffer:
+        """d_table [vocab, dim] of `embedding` (agpu_embedding_backward)."""
+        return self._new(_lib.load().agpu_embedding_backward, grad_out.handle, ids.handle, tokens,
+                         vocab, dim, C.c_float(scale))
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, positions, batch: int, seq: int,
+                     q_heads: int, k_heads: int, dim: int, rot_dim=None, eps: float = 1e-6,
+                     base: float = 10000.0, head_major: bool = False):
+        """RMSNorm of every query / key head, then the rotary embedding
+        (agpu_qk_norm_rope_forward) -> (q_out, k_out); an output without heads
+        is None.  Weights and positions may be None."""
+        return self._pair(_lib.load().agpu_qk_norm_rope_forward,
+                          (q, k, q_weight, k_weight, positions),
+                          (batch, seq, q_heads, k_heads, dim, dim if rot_dim is None else rot_dim,
+                           C.c_float(eps), C.c_float(base), int(head_major)), 2)
+
+    def qk_norm_rope_backward(self, d_q_out, d_k_out, q, k, q_weight, k_weight, positions,
+                              batch: int, seq: int, q_heads: int, k_heads: int, dim: int,
+                              rot_dim=None, eps: float = 1e-6, base: float = 10000.0,
+                              head_major: bool = False):
+        """(d_q, d_k, d_q_weight, d_k_weight) of `qk_norm_rope`
+        (agpu_qk_norm_rope_backward)."""
+        return self._pair(_lib.load().agpu_qk_norm_rope_backward,
+                          (d_q_out, d_k_out, q, k, q_weight, k_weight, positions),
+                          (batch, seq, q_heads, k_heads, dim, dim if rot_dim is None else rot_dim,
+                           C.c_float(eps), C.c_float(base), int(head_major)), 4)
+
+    def _pair(self, fn, bufs, args, n_out: int):
+        outs = [C.c_void_p() for _ in range(n_out)]
+        _check(fn(self._h, *[b.handle if b is not None else None for b in bufs], *args,
+                  *[C.byref(o) for o in outs]))
+        return tuple(GpuBuffer(o.value, self) if o.value else None for o in outs)
+
+    def orthogonalize(self, x, batch: int, rows: int, cols: int, steps: int = 5) -> GpuBuffer:
+        """Newton-Schulz iteration of each [rows, cols] matrix (agpu_orthogonalize)."""
+        return self._new(_lib.load().agpu_orthogonalize, x.handle, batch, rows, cols, steps)
+
+    def launch_embedding(self, table_ptr, ids_ptr, out_ptr, tokens, vocab, dim, scale=1.0,
+                         stream: int = 0) -> None:
+        _check(_lib.load().agpu_launch_embedding(self._h, table_ptr, ids_ptr, out_ptr, tokens,
+                                                 vocab, dim, C.c_float(scale), stream or None))
+
+    def launch_embedding_backward(self, grad_ptr, ids_ptr, d_table_ptr, tokens, vocab, dim,
+                                  scale=1.0, accumulate=False, stream: int = 0) -> None:
+        _check(_lib.load().agpu_launch_embedding_backward(
+            self._h, grad_ptr, ids_ptr, d_table_ptr, tokens, vocab, dim, C.c_float(scale),
+            int(accumulate), stream or None))
+
+    def launch_qk_norm_rope(self, shape, q_ptr, k_ptr, q_weight_ptr, k_weight_ptr, positions_ptr,
+                            q_out_ptr, k_out_ptr, stream: int = 0) -> None:
+        """`shape` from QkNormRope(...); weight and position pointers may be 0."""
+        _check(_lib.load().agpu_launch_qk_norm_rope(
+            self._h, C.byref(shape), q_ptr or None, k_ptr or None, q_weight_ptr or None,
+            k_weight_ptr or None, positions_ptr or None, q_out_ptr or None, k_out_ptr or None,
+            stream or None))
+
+    def launch_qk_norm_rope_backward(self, shape, d_q_out_ptr, d_k_out_ptr, q_ptr, k_ptr,
+                                     q_weight_ptr, k_weight_ptr, positions_ptr, d_q_ptr, d_k_ptr,
+                                     d_q_weight_ptr=0, d_k_weight_ptr=0,
+                                     stream: int = 0) -> None:
+        _check(_lib.load().agpu_launch_qk_norm_rope_backward(
+            self._h, C.byref(shape), d_q_out_ptr or None, d_k_out_ptr or None, q_ptr or None,
+            k_ptr or None, q_weight_ptr or None, k_weight_ptr or None, positions_ptr or None,
+            d_q_ptr or None, d_k_ptr or None, d_q_weight_ptr or None, d_k_weight_ptr or None,
+            stream or None))
+
+    def launch_orthogonalize(self, x_ptr, out_ptr, batch, rows, cols, steps=5,
+                             stream: int = 0) -> None:
+        _check(_lib.load().agpu_launch_orthogonalize(self._h, x_ptr, out_ptr, batch, rows, cols,
+                                                     steps, stream or None))
+
+    def launch_muon(self, tensors, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+                    stream: int = 0) -> None:
+        """One step for the matrices of `tensors` (from muon_tensors)."""
+        _check(_lib.load().agpu_launch_muon(self._h, C.addressof(tensors), len(tensors),
+                                            C.c_float(lr), C.c_float(momentum), int(nesterov),
+                                            C.c_float(weight_decay), steps, stream or None))
+
     # --------------------------------------------------------- elementwise --
     def add(self, a, b): return self._new(_lib.load().agpu_add, a.handle, b.handle)
     def sub(self, a, b): return self._new(_lib.load().agpu_sub, a.handle, b.handle)
@@ -530,3 +651,30 @@ class AdamW:
             arr([s[1] for s in self.states[:k]]), k, C.c_float(self.lr), C.c_float(self.beta1),
             C.c_float(self.beta2), C.c_float(self.eps), C.c_float(self.weight_decay),
             self.step_count))
+
+
+class Muon:
+    """Optimiser for the matrices of a model (agpu_muon_step): momentum, the
+    update orthogonalised by Newton-Schulz, decoupled weight decay.  Beside
+    AdamW: embeddings, norms and biases stay with that one, at the same
+    learning rate.  Momentum buffers are created (zero) on the first step."""
+
+    def __init__(self, lr: float, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.01, steps: int = 5):
+        self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
+        self.weight_decay, self.steps = weight_decay, steps
+        self.states: list[GpuBuffer] = []
+
+    def step(self, dev: "GpuDevice", params: list, grads: list, shapes: list) -> None:
+        """`shapes`: (rows, cols) of each parameter."""
+        k = len(params)
+        if len(grads) != k or len(shapes) != k:
+            raise AnyGpuError(1, "params/grads/shapes length mismatch")
+        while len(self.states) < k:
+            self.states.append(dev.alloc(params[len(self.states)].len))  # zero-filled
+        arr = lambda bufs: (C.c_void_p * max(k, 1))(*[b.handle for b in bufs])
+        dim = lambda i: (C.c_uint32 * max(k, 1))(*[s[i] for s in shapes])
+        _check(_lib.load().agpu_muon_step(
+            dev._h, arr(params), arr(grads), arr(self.states[:k]), dim(0), dim(1), k,
+            C.c_float(self.lr), C.c_float(self.momentum), int(self.nesterov),
+            C.c_float(self.weight_decay), self.steps))

@@ -37,6 +37,7 @@ SIGNATURES: dict[str, tuple] = {
     "agpu_upload": (c_status, [c_dev, C.c_void_p, u64, P_buf]),
     "agpu_alloc": (c_status, [c_dev, u64, P_buf]),
     "agpu_read": (c_status, [c_dev, c_buf, C.c_void_p, u64]),
+    "agpu_upload_i32": (c_status, [c_dev, C.c_void_p, u64, P_buf]),
     "agpu_write": (c_status, [c_dev, c_buf, C.c_void_p, u64]),
     "agpu_write_async": (c_status, [c_dev, c_buf, u64, C.c_void_p, u64, C.c_void_p]),
     "agpu_read_async": (c_status, [c_dev, c_buf, u64, C.c_void_p, u64, C.c_void_p]),
@@ -70,6 +71,12 @@ SIGNATURES: dict[str, tuple] = {
     "agpu_rmsnorm": (c_status, [c_dev, c_buf, c_buf, u32, u32, f32, P_buf]),
     "agpu_rope": (c_status, [c_dev, c_buf, u32, u32, u32, u32, f32, P_buf]),
     "agpu_swish_mul": (c_status, [c_dev, c_buf, c_buf, P_buf]),
+    "agpu_embedding": (c_status, [c_dev, c_buf, c_buf, u64, u32, u32, f32, P_buf]),
+    "agpu_embedding_backward": (c_status, [c_dev, c_buf, c_buf, u64, u32, u32, f32, P_buf]),
+    "agpu_qk_norm_rope_forward": (c_status, [c_dev] + [c_buf] * 5 + [u32] * 6
+                                  + [f32, f32, i32, P_buf, P_buf]),
+    "agpu_qk_norm_rope_backward": (c_status, [c_dev] + [c_buf] * 7 + [u32] * 6
+                                   + [f32, f32, i32] + [P_buf] * 4),
     "agpu_add": (c_status, [c_dev, c_buf, c_buf, P_buf]),
     "agpu_sub": (c_status, [c_dev, c_buf, c_buf, P_buf]),
     "agpu_mul": (c_status, [c_dev, c_buf, c_buf, P_buf]),
@@ -111,6 +118,13 @@ SIGNATURES: dict[str, tuple] = {
                         [u32, f32, f32, f32, f32, f32, u32]),
     "agpu_launch_adamw": (c_status, [c_dev, C.c_void_p, u32, f32, f32, f32, f32, f32, u32,
                                      C.c_void_p]),
+    "agpu_orthogonalize": (c_status, [c_dev, c_buf, u32, u32, u32, u32, P_buf]),
+    "agpu_muon_step": (c_status, [c_dev] + [C.POINTER(C.c_void_p)] * 3 + [C.POINTER(u32)] * 2
+                       + [u32, f32, f32, i32, f32, u32]),
+    "agpu_launch_muon": (c_status, [c_dev, C.c_void_p, u32, f32, f32, i32, f32, u32,
+                                    C.c_void_p]),
+    "agpu_launch_orthogonalize": (c_status, [c_dev, C.c_void_p, C.c_void_p, u32, u32, u32, u32,
+                                             C.c_void_p]),
     "agpu_launch_sdpa": (c_status, [c_dev] + [C.c_void_p] * 4 + [u32, u32, u32, i32,
                                                                  C.c_void_p]),
     "agpu_launch_sdpa_backward": (c_status, [c_dev] + [C.c_void_p] * 7 + [u32, u32, u32, i32,
@@ -125,6 +139,12 @@ SIGNATURES: dict[str, tuple] = {
     "agpu_launch_swish_mul": (c_status, [c_dev] + [C.c_void_p] * 3 + [u64, u32, u64, u64, u64,
                                                                       C.c_void_p]),
     "agpu_launch_softmax": (c_status, [c_dev, C.c_void_p, C.c_void_p, u64, u32, C.c_void_p]),
+    "agpu_launch_embedding": (c_status, [c_dev] + [C.c_void_p] * 3 + [u64, u32, u32, f32,
+                                                                      C.c_void_p]),
+    "agpu_launch_embedding_backward": (c_status, [c_dev] + [C.c_void_p] * 3
+                                       + [u64, u32, u32, f32, i32, C.c_void_p]),
+    "agpu_launch_qk_norm_rope": (c_status, [c_dev] + [C.c_void_p] * 9),
+    "agpu_launch_qk_norm_rope_backward": (c_status, [c_dev] + [C.c_void_p] * 13),
     "agpu_group_norm_noalloc": (c_status, [C.c_void_p] * 4 + [u32, u32, u32, u32, f32, i32,
                                                               C.c_void_p]),
     "agpu_ipc_export": (c_status, [c_dev, C.c_void_p, C.c_void_p, C.POINTER(u64)]),
@@ -144,6 +164,19 @@ SIGNATURES: dict[str, tuple] = {
 class AttnLayout(C.Structure):
     """agpu_attn_layout: element strides of one attention operand."""
     _fields_ = [("seq_stride", u64), ("head_stride", u64), ("batch_stride", u64)]
+
+
+class QkNormRopeShape(C.Structure):
+    """agpu_qk_norm_rope: geometry of the head norms with the rotary embedding."""
+    _fields_ = ([(n, u32) for n in ("batch", "seq", "q_heads", "k_heads", "dim", "rot_dim")]
+                + [("eps", f32), ("base", f32)]
+                + [(n, AttnLayout) for n in ("q_in", "k_in", "q_out", "k_out")])
+
+
+class MuonTensor(C.Structure):
+    """agpu_muon_tensor: one matrix of an orthogonalised-update step."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p),
+                ("rows", u32), ("cols", u32)]
 
 
 _LIB = None

@@ -26,6 +26,12 @@ fused attention forward as one op; its backward (`agpu_sdpa_backward`) is the
 reference's SDPA composition (src/ops/attention.rs:149-169) differentiated
 with its matmul and scale rules and the softmax Jacobian.
 
+Three more serve models over tokens: `embedding` (ids are an `upload_i32`
+buffer, not a tensor of the tape), `qk_norm_rope` (RMSNorm of every query and
+key head and the rotary embedding in one pass; two outputs) and `transpose`,
+which brings value heads into the [batch, heads, seq, dim] order of the other
+two attention operands.
+
 Gradients are accumulated with `add` into a fresh buffer (:267-279); the
 pass-through gradients of Add, Sub and the broadcast adds share the upstream
 buffer instead of copying it (buffers are never written after creation).
@@ -193,6 +199,33 @@ class Tape:
         return self._push(out, "sdpa", q=q, k=k, v=v, bh=batch_heads, s=seq_len, d=d_k,
                           causal=causal)
 
+    def embedding(self, table, ids: GpuBuffer, tokens: int, vocab: int, dim: int,
+                  scale: float = 1.0):
+        """scale * table[ids]; ids from `dev.upload_i32`, -1 = padding."""
+        out = self.dev.embedding(self.buf(table), ids, tokens, vocab, dim, scale)
+        return self._push(out, "embedding", table=table, ids=ids, tokens=tokens, vocab=vocab,
+                          dim=dim, scale=scale)
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, positions: Optional[GpuBuffer], batch: int,
+                     seq: int, q_heads: int, k_heads: int, dim: int, rot_dim=None,
+                     eps: float = 1e-6, base: float = 10000.0, head_major: bool = False):
+        """RMSNorm of every head of q and k, then the rotary embedding, as one
+        recorded op with two outputs (q_out, k_out).  Weights may be None;
+        positions (from `dev.upload_i32`) None = the sequence index."""
+        opt = lambda t: None if t is None else self.buf(t)
+        qo, ko = self.dev.qk_norm_rope(self.buf(q), self.buf(k), opt(q_weight), opt(k_weight),
+                                       positions, batch, seq, q_heads, k_heads, dim, rot_dim, eps,
+                                       base, head_major)
+        geometry = (batch, seq, q_heads, k_heads, dim, rot_dim, eps, base, head_major)
+        first = self._push(qo, "qk_norm_rope", q=q, k=k, q_weight=q_weight, k_weight=k_weight,
+                           positions=positions, geometry=geometry)
+        return first, self._push(ko, "qk_norm_rope_keys")
+
+    def transpose(self, a, outer: int, d0: int, d1: int, inner: int):
+        """[outer, d0, d1, inner] -> [outer, d1, d0, inner]."""
+        out = self.dev.transpose(self.buf(a), outer, d0, d1, inner)
+        return self._push(out, "transpose", a=a, outer=outer, d0=d0, d1=d1, inner=inner)
+
     # ----------------------------------------------------------- backward --
     def backward(self, loss: TensorId) -> None:
         """Gradients of every recorded tensor w.r.t. the 1-element `loss`
@@ -204,9 +237,12 @@ class Tape:
         self._grads[loss.index] = d.upload(np.ones(1, np.float32))
         for e in reversed(self._entries):
             g = self._grads[e.output.index]
-            if g is None or e.op == "leaf":
-                continue
             a = e.args
+            if e.op == "qk_norm_rope":  # its keys' entry follows it: both gradients are here
+                self._qk_norm_rope_backward(g, self._grads[e.output.index + 1], a)
+                continue
+            if g is None or e.op in ("leaf", "qk_norm_rope_keys"):
+                continue
             if e.op == "add":
                 self._accum(a["a"], g)
                 self._accum(a["b"], g)
@@ -280,8 +316,27 @@ class Tape:
                 self._accum(a["q"], dq)
                 self._accum(a["k"], dk)
                 self._accum(a["v"], dv)
+            elif e.op == "embedding":
+                self._accum(a["table"], d.embedding_backward(g, a["ids"], a["tokens"],
+                                                             a["vocab"], a["dim"], a["scale"]))
+            elif e.op == "transpose":
+                self._accum(a["a"], d.transpose(g, a["outer"], a["d1"], a["d0"], a["inner"]))
             else:  # pragma: no cover - every recorded op is handled above
                 raise KeyError(e.op)
+
+    def _qk_norm_rope_backward(self, gq: Optional[GpuBuffer], gk: Optional[GpuBuffer],
+                               a: Dict) -> None:
+        if gq is None and gk is None:
+            return
+        d = self.dev
+        q, k, qw, kw = (None if a[n] is None else self.buf(a[n])
+                        for n in ("q", "k", "q_weight", "k_weight"))
+        gq = d.alloc(q.len) if gq is None else gq  # zeros: an output nothing used
+        gk = d.alloc(k.len) if gk is None else gk
+        grads = d.qk_norm_rope_backward(gq, gk, q, k, qw, kw, a["positions"], *a["geometry"])
+        for name, g in zip(("q", "k", "q_weight", "k_weight"), grads):
+            if a[name] is not None:
+                self._accum(a[name], g)
 
     def _conv2d_backward(self, g: GpuBuffer, a: Dict) -> None:
         d = self.dev

@@ -5,7 +5,9 @@ pointers, one stream); this module only sequences the launches:
 
     h1  = rmsnorm(x, w_attn_norm)                       [T, d]      T = B*S
     qkv = h1 @ Wqkv                                     [T, 3d]     packed [B,S,3,H,Dh]
-    q,k = rope(q), rope(k)       (in place, positions = sequence index)
+    q,k = rope(q), rope(k)       (in place, positions = sequence index; with
+                                  qk_norm, every head is RMS-normed first, in
+                                  the same pass over q and k)
     o   = sdpa(q, k, v)          (strided: read straight from qkv, written [B,S,H,Dh])
     x2  = x + o @ Wo             (residual fused in the GEMM epilogue)
     h2  = rmsnorm(x2, w_ffn_norm)
@@ -23,6 +25,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+from . import QkNormRope
+
 F32 = 4
 
 
@@ -36,6 +40,7 @@ class LlamaDims:
     eps: float = 1e-5
     rope_base: float = 10000.0
     causal: bool = False
+    qk_norm: bool = False
 
     @property
     def tokens(self) -> int:
@@ -67,16 +72,22 @@ class LlamaDims:
 
 def layer_forward(dev, dims: LlamaDims, x, w, ws, y, stream: int = 0) -> None:
     """x, y: device pointers [T, d]; w: dict of weight pointers (attn_norm [d],
-    wqkv [d,3d], wo [d,d], ffn_norm [d], wgu [d,2F], wd [F,d]); ws: dict of
-    workspace pointers sized by dims.workspace_elems()."""
+    wqkv [d,3d], wo [d,d], ffn_norm [d], wgu [d,2F], wd [F,d], and with
+    dims.qk_norm q_norm and k_norm [head_dim]); ws: dict of workspace pointers
+    sized by dims.workspace_elems()."""
     B, S, d, H, Fd = dims.batch, dims.seq, dims.d_model, dims.heads, dims.ffn
     T, Dh = dims.tokens, dims.head_dim
     dev.launch_rmsnorm(x, w["attn_norm"], ws["h"], T, d, dims.eps, stream)
     dev.launch_gemm_ex(ws["h"], w["wqkv"], ws["qkv"], 1, T, 3 * d, d, stream=stream)
     q, k, v = ws["qkv"], ws["qkv"] + d * F32, ws["qkv"] + 2 * d * F32
-    dev.launch_rope(q, q, B, S, H, Dh, 3 * d, dims.rope_base, stream)
-    dev.launch_rope(k, k, B, S, H, Dh, 3 * d, dims.rope_base, stream)
     qkv_st = (3 * d, Dh, S * 3 * d)
+    if dims.qk_norm:
+        shape = QkNormRope(B, S, H, H, Dh, eps=dims.eps, base=dims.rope_base, q_in=qkv_st,
+                           k_in=qkv_st, q_out=qkv_st, k_out=qkv_st)
+        dev.launch_qk_norm_rope(shape, q, k, w["q_norm"], w["k_norm"], 0, q, k, stream)
+    else:
+        dev.launch_rope(q, q, B, S, H, Dh, 3 * d, dims.rope_base, stream)
+        dev.launch_rope(k, k, B, S, H, Dh, 3 * d, dims.rope_base, stream)
     o_st = (d, Dh, S * d)
     dev.launch_sdpa_strided(q, k, v, ws["o"], B, H, S, Dh, qkv_st, qkv_st, qkv_st, o_st,
                             dims.causal, stream)

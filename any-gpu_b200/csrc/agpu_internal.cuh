@@ -39,6 +39,7 @@ struct agpu_buffer {
   float* dptr = nullptr;
   uint64_t len = 0;
   agpu_device* dev = nullptr;
+  bool i32 = false;  // holds int32 values (agpu_upload_i32): token ids, positions
 };
 
 namespace agpu {
@@ -164,6 +165,31 @@ agpu_status launch_rope(agpu_device* dev, const float* x, float* y, uint32_t bat
 agpu_status launch_swish_mul(agpu_device* dev, const float* gate, const float* up, float* out,
                              uint64_t rows, uint32_t cols, uint64_t gs, uint64_t us, uint64_t os,
                              cudaStream_t s);
+// Token embedding and its gradient; ids on the device, -1 = padding.
+agpu_status launch_embedding(agpu_device* dev, const float* table, const int32_t* ids, float* out,
+                             uint64_t tokens, uint32_t vocab, uint32_t dim, float scale,
+                             cudaStream_t s);
+agpu_status launch_embedding_backward(agpu_device* dev, const float* grad_out, const int32_t* ids,
+                                      float* d_table, uint64_t tokens, uint32_t vocab,
+                                      uint32_t dim, float scale, bool accumulate, cudaStream_t s);
+// Head norms with the rotary embedding, and the gradients (weights' gradients
+// may be null).
+agpu_status launch_qk_norm_rope(agpu_device* dev, const agpu_qk_norm_rope& d, const float* q,
+                                const float* k, const float* q_weight, const float* k_weight,
+                                const int32_t* positions, float* q_out, float* k_out,
+                                cudaStream_t s);
+agpu_status launch_qk_norm_rope_backward(agpu_device* dev, const agpu_qk_norm_rope& d,
+                                         const float* d_q_out, const float* d_k_out,
+                                         const float* q, const float* k, const float* q_weight,
+                                         const float* k_weight, const int32_t* positions,
+                                         float* d_q, float* d_k, float* d_q_weight,
+                                         float* d_k_weight, cudaStream_t s);
+// Newton-Schulz orthogonalisation and the optimiser step on it.
+agpu_status launch_orthogonalize(agpu_device* dev, const float* x, float* out, uint32_t batch,
+                                 uint32_t rows, uint32_t cols, uint32_t steps, cudaStream_t s);
+agpu_status launch_muon(agpu_device* dev, const agpu_muon_tensor* tensors, uint32_t count,
+                        float lr, float momentum, bool nesterov, float weight_decay,
+                        uint32_t steps, cudaStream_t s);
 agpu_status launch_attention_strided(agpu_device* dev, const float* q, const float* k,
                                      const float* v, float* o, uint32_t B, uint32_t H,
                                      uint32_t s, uint32_t d, const long long (&qs)[3],

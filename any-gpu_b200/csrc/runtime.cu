@@ -105,6 +105,8 @@ agpu_status check_device_status(agpu_device* dev) {
   AGPU_CUDA(cudaStreamSynchronize(dev->stream));
   if (h != 0) {
     AGPU_CUDA(cudaMemsetAsync(dev->d_status, 0, sizeof(unsigned int), dev->stream));
+    if (h == AGPU_BAD_TOKEN_CODE)
+      return fail(AGPU_ERR_INVALID, "a token id was outside its embedding table (code 0x%x)", h);
     return fail(AGPU_ERR_TIMEOUT, "a device-side bounded wait expired (code 0x%x)", h);
   }
   return AGPU_OK;
@@ -278,6 +280,14 @@ agpu_status agpu_upload(agpu_device* dev, const float* host, uint64_t n, agpu_bu
       return cuda_status(e, "agpu_upload");
     }
   }
+  return AGPU_OK;
+}
+
+agpu_status agpu_upload_i32(agpu_device* dev, const int32_t* host, uint64_t n,
+                            agpu_buffer** out) {
+  static_assert(sizeof(int32_t) == sizeof(float), "buffers hold 4-byte elements");
+  AGPU_TRY(agpu_upload(dev, reinterpret_cast<const float*>(host), n, out));
+  (*out)->i32 = true;
   return AGPU_OK;
 }
 

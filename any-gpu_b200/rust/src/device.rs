@@ -497,6 +497,81 @@ impl GpuDevice {
         self.out(|o| unsafe { ffi::agpu_swish_mul(self.raw, gate.c(), up.c(), o) })
     }
 
+    // ------------------------------------------ ops for training on tokens --
+    /// int32 values (token ids, positions) in a buffer of their own kind.
+    pub fn upload_i32(&self, data: &[i32]) -> Result<GpuBuffer> {
+        self.out(|o| unsafe {
+            ffi::agpu_upload_i32(self.raw, data.as_ptr(), data.len() as u64, o)
+        })
+    }
+    /// out[t] = scale * table[ids[t]]; id -1 is padding (a zero row).
+    pub fn embedding(
+        &self, table: &GpuBuffer, ids: &GpuBuffer, tokens: u64, vocab: u32, dim: u32, scale: f32,
+    ) -> Result<GpuBuffer> {
+        self.out(|o| unsafe {
+            ffi::agpu_embedding(self.raw, table.c(), ids.c(), tokens, vocab, dim, scale, o)
+        })
+    }
+    /// The gradient of `embedding` with respect to its table.
+    pub fn embedding_backward(
+        &self, grad_out: &GpuBuffer, ids: &GpuBuffer, tokens: u64, vocab: u32, dim: u32,
+        scale: f32,
+    ) -> Result<GpuBuffer> {
+        self.out(|o| unsafe {
+            ffi::agpu_embedding_backward(self.raw, grad_out.c(), ids.c(), tokens, vocab, dim,
+                                         scale, o)
+        })
+    }
+    /// RMSNorm of every head of `q`, then the rotary embedding (one operand of
+    /// the fused pass; call it with `q_heads` and `k_heads` through `ffi` for both).
+    #[allow(clippy::too_many_arguments)]
+    pub fn norm_rope(
+        &self, q: &GpuBuffer, weight: Option<&GpuBuffer>, positions: Option<&GpuBuffer>,
+        batch: u32, seq: u32, heads: u32, dim: u32, rot_dim: u32, eps: f32, base: f32,
+        head_major: bool,
+    ) -> Result<GpuBuffer> {
+        self.out(|o| unsafe {
+            ffi::agpu_qk_norm_rope_forward(self.raw, q.c(), ptr::null(), opt(weight), ptr::null(),
+                                           opt(positions), batch, seq, heads, 0, dim, rot_dim,
+                                           eps, base, head_major as c_int, o, ptr::null_mut())
+        })
+    }
+    /// Newton-Schulz iteration of each [rows, cols] matrix.
+    pub fn orthogonalize(
+        &self, x: &GpuBuffer, batch: u32, rows: u32, cols: u32, steps: u32,
+    ) -> Result<GpuBuffer> {
+        self.out(|o| unsafe {
+            ffi::agpu_orthogonalize(self.raw, x.c(), batch, rows, cols, steps, o)
+        })
+    }
+    /// One orthogonalised-update step over many matrices; params and momenta
+    /// are updated in place; `shapes` holds (rows, cols).
+    #[allow(clippy::too_many_arguments)]
+    pub fn muon_step(
+        &self, params: &[&GpuBuffer], grads: &[&GpuBuffer], momenta: &[&GpuBuffer],
+        shapes: &[(u32, u32)], lr: f32, momentum: f32, nesterov: bool, weight_decay: f32,
+        steps: u32,
+    ) -> Result<()> {
+        let n = params.len();
+        if grads.len() != n || momenta.len() != n || shapes.len() != n {
+            return Err(AgpuError {
+                status: ffi::AGPU_ERR_SHAPE,
+                message: "muon_step: params, grads, momenta and shapes differ in count".to_string(),
+            }
+            .into());
+        }
+        let p: Vec<*mut ffi::AgpuBuffer> = params.iter().map(|b| b.raw).collect();
+        let g: Vec<*const ffi::AgpuBuffer> = grads.iter().map(|b| b.c()).collect();
+        let m: Vec<*mut ffi::AgpuBuffer> = momenta.iter().map(|b| b.raw).collect();
+        let rows: Vec<u32> = shapes.iter().map(|s| s.0).collect();
+        let cols: Vec<u32> = shapes.iter().map(|s| s.1).collect();
+        check(unsafe {
+            ffi::agpu_muon_step(self.raw, p.as_ptr(), g.as_ptr(), m.as_ptr(), rows.as_ptr(),
+                                cols.as_ptr(), n as u32, lr, momentum, nesterov as c_int,
+                                weight_decay, steps)
+        })
+    }
+
     // -------------------------------------------------------------- AdamW --
     /// One AdamW step over many tensors in one launch (the reference's
     /// `AdamW::step`, src/optim.rs:82-138); params, m and v are updated in

@@ -67,6 +67,38 @@ pub struct AgpuAdamwTensor {
     pub n: u64,
 }
 
+/// `AGPU_BAD_TOKEN_CODE`: the status code of a token id outside its table.
+pub const AGPU_BAD_TOKEN_CODE: u32 = 0x7091;
+
+/// `agpu_qk_norm_rope`: geometry of the head norms with the rotary embedding.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct AgpuQkNormRope {
+    pub batch: u32,
+    pub seq: u32,
+    pub q_heads: u32,
+    pub k_heads: u32,
+    pub dim: u32,
+    pub rot_dim: u32,
+    pub eps: f32,
+    pub base: f32,
+    pub q_in: AgpuAttnLayout,
+    pub k_in: AgpuAttnLayout,
+    pub q_out: AgpuAttnLayout,
+    pub k_out: AgpuAttnLayout,
+}
+
+/// `agpu_muon_tensor`: one matrix of an orthogonalised-update step.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct AgpuMuonTensor {
+    pub param: *mut f32,
+    pub grad: *const f32,
+    pub momentum: *mut f32,
+    pub rows: u32,
+    pub cols: u32,
+}
+
 #[link(name = "agpu")]
 extern "C" {
     pub fn agpu_last_error_message() -> *const c_char;
@@ -99,6 +131,12 @@ extern "C" {
         buf: *const AgpuBuffer,
         host: *mut f32,
         n: u64,
+    ) -> AgpuStatus;
+    pub fn agpu_upload_i32(
+        dev: *mut AgpuDevice,
+        host: *const i32,
+        n: u64,
+        out: *mut *mut AgpuBuffer,
     ) -> AgpuStatus;
     pub fn agpu_write(
         dev: *mut AgpuDevice,
@@ -385,6 +423,68 @@ extern "C" {
         up: *const AgpuBuffer,
         out: *mut *mut AgpuBuffer,
     ) -> AgpuStatus;
+    pub fn agpu_embedding(
+        dev: *mut AgpuDevice,
+        table: *const AgpuBuffer,
+        ids: *const AgpuBuffer,
+        tokens: u64,
+        vocab: u32,
+        dim: u32,
+        scale: f32,
+        out: *mut *mut AgpuBuffer,
+    ) -> AgpuStatus;
+    pub fn agpu_embedding_backward(
+        dev: *mut AgpuDevice,
+        grad_out: *const AgpuBuffer,
+        ids: *const AgpuBuffer,
+        tokens: u64,
+        vocab: u32,
+        dim: u32,
+        scale: f32,
+        d_table: *mut *mut AgpuBuffer,
+    ) -> AgpuStatus;
+    pub fn agpu_qk_norm_rope_forward(
+        dev: *mut AgpuDevice,
+        q: *const AgpuBuffer,
+        k: *const AgpuBuffer,
+        q_weight: *const AgpuBuffer,
+        k_weight: *const AgpuBuffer,
+        positions: *const AgpuBuffer,
+        batch: u32,
+        seq: u32,
+        q_heads: u32,
+        k_heads: u32,
+        dim: u32,
+        rot_dim: u32,
+        eps: f32,
+        base: f32,
+        head_major: c_int,
+        q_out: *mut *mut AgpuBuffer,
+        k_out: *mut *mut AgpuBuffer,
+    ) -> AgpuStatus;
+    pub fn agpu_qk_norm_rope_backward(
+        dev: *mut AgpuDevice,
+        d_q_out: *const AgpuBuffer,
+        d_k_out: *const AgpuBuffer,
+        q: *const AgpuBuffer,
+        k: *const AgpuBuffer,
+        q_weight: *const AgpuBuffer,
+        k_weight: *const AgpuBuffer,
+        positions: *const AgpuBuffer,
+        batch: u32,
+        seq: u32,
+        q_heads: u32,
+        k_heads: u32,
+        dim: u32,
+        rot_dim: u32,
+        eps: f32,
+        base: f32,
+        head_major: c_int,
+        d_q: *mut *mut AgpuBuffer,
+        d_k: *mut *mut AgpuBuffer,
+        d_q_weight: *mut *mut AgpuBuffer,
+        d_k_weight: *mut *mut AgpuBuffer,
+    ) -> AgpuStatus;
     pub fn agpu_add(
         dev: *mut AgpuDevice,
         a: *const AgpuBuffer,
@@ -562,6 +662,50 @@ extern "C" {
         eps: f32,
         weight_decay: f32,
         step: u32,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_orthogonalize(
+        dev: *mut AgpuDevice,
+        x: *const AgpuBuffer,
+        batch: u32,
+        rows: u32,
+        cols: u32,
+        steps: u32,
+        out: *mut *mut AgpuBuffer,
+    ) -> AgpuStatus;
+    pub fn agpu_muon_step(
+        dev: *mut AgpuDevice,
+        params: *const *mut AgpuBuffer,
+        grads: *const *const AgpuBuffer,
+        momenta: *const *mut AgpuBuffer,
+        rows: *const u32,
+        cols: *const u32,
+        count: u32,
+        lr: f32,
+        momentum: f32,
+        nesterov: c_int,
+        weight_decay: f32,
+        steps: u32,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_muon(
+        dev: *mut AgpuDevice,
+        tensors: *const AgpuMuonTensor,
+        count: u32,
+        lr: f32,
+        momentum: f32,
+        nesterov: c_int,
+        weight_decay: f32,
+        steps: u32,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_orthogonalize(
+        dev: *mut AgpuDevice,
+        x: *const f32,
+        out: *mut f32,
+        batch: u32,
+        rows: u32,
+        cols: u32,
+        steps: u32,
         stream: *mut c_void,
     ) -> AgpuStatus;
     pub fn agpu_launch_batch_matmul(
@@ -776,6 +920,57 @@ extern "C" {
         y: *mut f32,
         rows: u64,
         cols: u32,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_embedding(
+        dev: *mut AgpuDevice,
+        table: *const f32,
+        ids: *const i32,
+        out: *mut f32,
+        tokens: u64,
+        vocab: u32,
+        dim: u32,
+        scale: f32,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_embedding_backward(
+        dev: *mut AgpuDevice,
+        grad_out: *const f32,
+        ids: *const i32,
+        d_table: *mut f32,
+        tokens: u64,
+        vocab: u32,
+        dim: u32,
+        scale: f32,
+        accumulate: c_int,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_qk_norm_rope(
+        dev: *mut AgpuDevice,
+        shape: *const AgpuQkNormRope,
+        q: *const f32,
+        k: *const f32,
+        q_weight: *const f32,
+        k_weight: *const f32,
+        positions: *const i32,
+        q_out: *mut f32,
+        k_out: *mut f32,
+        stream: *mut c_void,
+    ) -> AgpuStatus;
+    pub fn agpu_launch_qk_norm_rope_backward(
+        dev: *mut AgpuDevice,
+        shape: *const AgpuQkNormRope,
+        d_q_out: *const f32,
+        d_k_out: *const f32,
+        q: *const f32,
+        k: *const f32,
+        q_weight: *const f32,
+        k_weight: *const f32,
+        positions: *const i32,
+        d_q: *mut f32,
+        d_k: *mut f32,
+        d_q_weight: *mut f32,
+        d_k_weight: *mut f32,
         stream: *mut c_void,
     ) -> AgpuStatus;
     pub fn agpu_group_norm_noalloc(

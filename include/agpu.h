@@ -123,6 +123,12 @@ AGPU_API agpu_status agpu_alloc(agpu_device* dev, uint64_t n, agpu_buffer** out)
  * whole buffer; `n` must equal the buffer length. */
 AGPU_API agpu_status agpu_read(agpu_device* dev, const agpu_buffer* buf, float* host,
                                uint64_t n);
+/* H2D copy of n int32 values (token ids, positions) into a new buffer of n
+ * 4-byte elements.  The ops below that take ids or positions accept only such
+ * buffers (else AGPU_ERR_INVALID); agpu_read returns their bytes.  No
+ * counterpart in the reference, whose buffers are all f32. */
+AGPU_API agpu_status agpu_upload_i32(agpu_device* dev, const int32_t* host, uint64_t n,
+                                     agpu_buffer** out);
 /* Stream-ordered H2D into an existing buffer (no new allocation). */
 AGPU_API agpu_status agpu_write(agpu_device* dev, agpu_buffer* buf, const float* host,
                                 uint64_t n);
@@ -325,6 +331,68 @@ AGPU_API agpu_status agpu_rope(agpu_device* dev, const agpu_buffer* x, uint32_t 
 AGPU_API agpu_status agpu_swish_mul(agpu_device* dev, const agpu_buffer* gate,
                                     const agpu_buffer* up, agpu_buffer** out);
 
+/* Element strides of one attention operand laid out as [batch, seq, heads, d]
+ * in any order (d contiguous): e.g. contiguous [bh, s, d] is
+ * {d, s*d, bh*s*d} with heads = bh, batch = 1; the Q part of a packed
+ * [batch, seq, 3, heads, d] projection is {3*heads*d, d, seq*3*heads*d}. */
+typedef struct agpu_attn_layout {
+  uint64_t seq_stride, head_stride, batch_stride;
+} agpu_attn_layout;
+
+/* --------------------------------------- ops for training on tokens ------- */
+/* No counterparts in the reference (its tape starts from dense leaves). */
+/* Embedding lookup: out[t] = scale * table[ids[t]], table [vocab, dim], ids an
+ * agpu_upload_i32 buffer of `tokens` ids, out [tokens, dim].  id -1 is padding:
+ * a zero row.  Ids are checked on the device: any other id outside [0, vocab)
+ * counts as padding and the next agpu_synchronize / agpu_read returns
+ * AGPU_ERR_INVALID. */
+#define AGPU_BAD_TOKEN_CODE 0x7091u
+AGPU_API agpu_status agpu_embedding(agpu_device* dev, const agpu_buffer* table,
+                                    const agpu_buffer* ids, uint64_t tokens, uint32_t vocab,
+                                    uint32_t dim, float scale, agpu_buffer** out);
+/* Its gradient: d_table[v] = scale * the sum of grad_out[t] over the tokens t
+ * with id v, [vocab, dim], zero rows for ids that do not occur.  Each row's
+ * sum has a fixed order, so the result is deterministic.  Pool scratch of
+ * about 8 bytes per token, 4 per table row, and 1/16 of grad_out. */
+AGPU_API agpu_status agpu_embedding_backward(agpu_device* dev, const agpu_buffer* grad_out,
+                                             const agpu_buffer* ids, uint64_t tokens,
+                                             uint32_t vocab, uint32_t dim, float scale,
+                                             agpu_buffer** d_table);
+/* Geometry of agpu_qk_norm_rope and its backward: q_heads query heads and
+ * k_heads key heads (either may be 0) of `dim` elements (1..1024) for
+ * batch * seq tokens; the first rot_dim elements of a head (even, 0..dim) are
+ * rotated.  Layouts: `_in` of q / k and their gradients, `_out` of q_out /
+ * k_out and theirs; the strides of a layout may come in any order but must
+ * not make elements overlap (AGPU_ERR_SHAPE). */
+typedef struct agpu_qk_norm_rope {
+  uint32_t batch, seq, q_heads, k_heads, dim, rot_dim;
+  float eps, base;
+  agpu_attn_layout q_in, k_in, q_out, k_out;
+} agpu_qk_norm_rope;
+/* RMSNorm of every head, then the rotary embedding, in one pass over q and k:
+ * y = x / sqrt(mean(x^2) + eps) * weight; element pairs (i, i + rot_dim/2) of
+ * y turned by position * base^(-2i/rot_dim) (rotate-half, as agpu_rope).
+ * q [batch, seq, q_heads, dim], k likewise; weights [dim] or NULL (ones);
+ * positions an agpu_upload_i32 buffer [batch, seq] or NULL (the sequence
+ * index).  head_major = 0: outputs laid out like the inputs; 1: as
+ * [batch, heads, seq, dim], what the attention ops take.  With k_heads = 0, k
+ * and k_out are NULL, and likewise for q. */
+AGPU_API agpu_status agpu_qk_norm_rope_forward(
+    agpu_device* dev, const agpu_buffer* q, const agpu_buffer* k, const agpu_buffer* q_weight,
+    const agpu_buffer* k_weight, const agpu_buffer* positions, uint32_t batch, uint32_t seq,
+    uint32_t q_heads, uint32_t k_heads, uint32_t dim, uint32_t rot_dim, float eps, float base,
+    int head_major, agpu_buffer** q_out, agpu_buffer** k_out);
+/* Its gradients from those of its outputs (laid out as the outputs); d_q and
+ * d_k are laid out like q and k.  d_q_weight / d_k_weight ([dim]) may be NULL
+ * pointers when not wanted; every sum has a fixed order. */
+AGPU_API agpu_status agpu_qk_norm_rope_backward(
+    agpu_device* dev, const agpu_buffer* d_q_out, const agpu_buffer* d_k_out,
+    const agpu_buffer* q, const agpu_buffer* k, const agpu_buffer* q_weight,
+    const agpu_buffer* k_weight, const agpu_buffer* positions, uint32_t batch, uint32_t seq,
+    uint32_t q_heads, uint32_t k_heads, uint32_t dim, uint32_t rot_dim, float eps, float base,
+    int head_major, agpu_buffer** d_q, agpu_buffer** d_k, agpu_buffer** d_q_weight,
+    agpu_buffer** d_k_weight);
+
 /* --------------------------------------------------------- elementwise ---- */
 /* src/ops/elementwise.rs:188-250.  Binary ops require equal lengths. */
 AGPU_API agpu_status agpu_add(agpu_device* dev, const agpu_buffer* a, const agpu_buffer* b,
@@ -428,6 +496,44 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
                                        float eps, float weight_decay, uint32_t step,
                                        void* stream);
 
+/* ------------------------------------------- orthogonalised updates ------- */
+/* No counterpart in the reference; for the matrices of a model, beside AdamW.
+ * The quintic Newton-Schulz iteration, which drives the singular values of a
+ * matrix towards 1: X = x / max(|x|_F, 1e-30), then `steps` times
+ *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X
+ * (on X^T when rows > cols).  x [batch, rows, cols], each matrix by itself.
+ * fp32-level accuracy whatever the precision mode.  steps 1..64, else
+ * AGPU_ERR_INVALID. */
+AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t batch,
+                                        uint32_t rows, uint32_t cols, uint32_t steps,
+                                        agpu_buffer** out);
+/* One optimiser step for `count` matrices, in place:
+ *   M <- momentum M + (1 - momentum) G
+ *   U = nesterov ? (1 - momentum) G + momentum M : M
+ *   W <- (1 - lr weight_decay) W - lr 0.2 sqrt(max(rows, cols)) orthogonalize(U)
+ * The factor gives an update the root mean square of an AdamW step, so both
+ * can share a learning rate.  rows / cols are host arrays; M starts at zero;
+ * a length other than rows * cols -> AGPU_ERR_SHAPE. */
+AGPU_API agpu_status agpu_muon_step(agpu_device* dev, agpu_buffer* const* params,
+                                    const agpu_buffer* const* grads, agpu_buffer* const* momenta,
+                                    const uint32_t* rows, const uint32_t* cols, uint32_t count,
+                                    float lr, float momentum, int nesterov, float weight_decay,
+                                    uint32_t steps);
+/* The same on caller-owned device memory: a host array of matrices. */
+typedef struct agpu_muon_tensor {
+  float* param;
+  const float* grad;
+  float* momentum;
+  uint32_t rows, cols;
+} agpu_muon_tensor;
+AGPU_API agpu_status agpu_launch_muon(agpu_device* dev, const agpu_muon_tensor* tensors,
+                                      uint32_t count, float lr, float momentum, int nesterov,
+                                      float weight_decay, uint32_t steps, void* stream);
+/* out may be x itself, but must not overlap it otherwise.  Pool scratch. */
+AGPU_API agpu_status agpu_launch_orthogonalize(agpu_device* dev, const float* x, float* out,
+                                               uint32_t batch, uint32_t rows, uint32_t cols,
+                                               uint32_t steps, void* stream);
+
 /* ------------------------------------------------ launch layer (raw ptrs) -- */
 /* Same kernels on caller-owned device memory; `stream` is a cudaStream_t
  * (NULL = the device's own stream).  No allocation happens in these calls
@@ -483,13 +589,6 @@ AGPU_API agpu_status agpu_launch_gemm_ex(agpu_device* dev, const float* a, const
                                          float* c, uint32_t batch, uint32_t m, uint32_t n,
                                          uint32_t k, int trans_a, int trans_b, const float* bias,
                                          const float* resid, int act, void* stream);
-/* Element strides of one attention operand laid out as [batch, seq, heads, d]
- * in any order (d contiguous): e.g. contiguous [bh, s, d] is
- * {d, s*d, bh*s*d} with heads = bh, batch = 1; the Q part of a packed
- * [batch, seq, 3, heads, d] projection is {3*heads*d, d, seq*3*heads*d}. */
-typedef struct agpu_attn_layout {
-  uint64_t seq_stride, head_stride, batch_stride;
-} agpu_attn_layout;
 AGPU_API agpu_status agpu_launch_sdpa_strided(agpu_device* dev, const float* q, const float* k,
                                               const float* v, float* out, uint32_t batch,
                                               uint32_t heads, uint32_t seq_len, uint32_t d_k,
@@ -512,6 +611,29 @@ AGPU_API agpu_status agpu_launch_swish_mul(agpu_device* dev, const float* gate, 
                                            uint64_t out_stride, void* stream);
 AGPU_API agpu_status agpu_launch_softmax(agpu_device* dev, const float* x, float* y,
                                          uint64_t rows, uint32_t cols, void* stream);
+AGPU_API agpu_status agpu_launch_embedding(agpu_device* dev, const float* table,
+                                           const int32_t* ids, float* out, uint64_t tokens,
+                                           uint32_t vocab, uint32_t dim, float scale,
+                                           void* stream);
+/* accumulate != 0: d_table += the gradient (rows without tokens untouched).
+ * Pool scratch as agpu_embedding_backward. */
+AGPU_API agpu_status agpu_launch_embedding_backward(agpu_device* dev, const float* grad_out,
+                                                    const int32_t* ids, float* d_table,
+                                                    uint64_t tokens, uint32_t vocab,
+                                                    uint32_t dim, float scale, int accumulate,
+                                                    void* stream);
+/* Outputs may be the inputs themselves where the layouts are equal. */
+AGPU_API agpu_status agpu_launch_qk_norm_rope(agpu_device* dev, const agpu_qk_norm_rope* shape,
+                                              const float* q, const float* k,
+                                              const float* q_weight, const float* k_weight,
+                                              const int32_t* positions, float* q_out,
+                                              float* k_out, void* stream);
+/* d_q_weight / d_k_weight may be NULL; pool scratch when they are not. */
+AGPU_API agpu_status agpu_launch_qk_norm_rope_backward(
+    agpu_device* dev, const agpu_qk_norm_rope* shape, const float* d_q_out, const float* d_k_out,
+    const float* q, const float* k, const float* q_weight, const float* k_weight,
+    const int32_t* positions, float* d_q, float* d_k, float* d_q_weight, float* d_k_weight,
+    void* stream);
 
 /* ------------------------------------------- allocation-free group norm -- */
 /* No counterpart in the reference.  Group norm (same math as agpu_group_norm,

@@ -1,0 +1,258 @@
+"""Orthogonalised updates against numpy in float64.
+
+Tolerances, relative in the Frobenius norm.
+
+TOL = 2e-5, for matrices whose singular values are spread like a gradient's
+(a few large ones on a floor of noise that the iteration lifts to 1 too).  One
+step maps a singular value s to s (a + b l + c l^2), l = s^2 <= 1.46; a relative
+error e of A = X X^T or of B = b A + c A^2 (against its largest eigenvalue)
+moves the result by at most 1.21 (|b| + 2 c 1.46) 1.46 e < 20 e.  The products
+keep 22 bits of each factor and sum in 32-bit accumulators: e <= 2^-20.
+
+DEGENERATE = 1.1e-3, for matrices with singular values that stay 0 (rank 1, a
+single entry).  What a step leaves in those directions is not moved towards 1
+but multiplied by the slope at 0, a = 3.4445, in every later step: by a^5 =
+485 from the initial rounding on.  Rounding X to 22 bits before each step:
+2^-22 (a^5 + a^4 + a^3 + a^2 + a) = 2^-22 685 = 1.6e-4.  An error e of A turns
+a large direction into a dead one, |b| e <= 4.775 2^-20 a step, and the steps
+behind it multiply that by 1 + a + ... + a^4 = 198: 9.0e-4."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+U = 2.0 ** -24
+TOL = 2e-5
+DEGENERATE = 1.1e-3
+A, B, CC = 3.4445, -4.7750, 2.0315
+gpu = pytest.mark.gpu
+
+
+def _orthogonalize(u, steps=5):
+    u = u.astype(np.float64)
+    x = u / max(np.linalg.norm(u), 1e-30)
+    tall = u.shape[0] > u.shape[1]
+    x = x.T if tall else x
+    for _ in range(steps):
+        g = x @ x.T
+        x = A * x + (B * g + CC * (g @ g)) @ x
+    return x.T if tall else x
+
+
+def _rel(got, want):
+    return np.linalg.norm(np.asarray(got, np.float64).ravel() - want.ravel()) / max(
+        np.linalg.norm(want), 1e-300)
+
+
+def _gradient(r, rows, cols):
+    """A decaying spectrum on top of noise."""
+    k = min(rows, cols, 16)
+    x = (r.standard_normal((rows, k)) * 0.7 ** np.arange(k)) @ r.standard_normal((k, cols))
+    return (x + 0.5 * r.standard_normal((rows, cols))).astype(np.float32)
+
+
+SHAPES = [(1, 1), (1, 9), (9, 1), (7, 5), (32, 32), (33, 129), (64, 256), (128, 128), (127, 127),
+          (130, 100), (129, 257), (256, 512), (200, 1000), (1000, 200), (255, 300), (513, 520),
+          (640, 384), (1024, 1031)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_orthogonalize(dev, rows, cols):
+    r = np.random.default_rng(rows * cols)
+    x = _gradient(r, rows, cols) * np.float32(1e-3)
+    X = dev.upload(x)
+    got = dev.read(dev.orthogonalize(X, 1, rows, cols))
+    assert _rel(got, _orthogonalize(x)) <= TOL
+    np.testing.assert_array_equal(dev.read(X).reshape(x.shape), x)  # the input is only read
+    np.testing.assert_array_equal(got, dev.read(dev.orthogonalize(X, 1, rows, cols)))
+
+
+@gpu
+@pytest.mark.parametrize("batch,rows,cols,steps", [(3, 40, 72, 1), (2, 130, 64, 3), (5, 256, 256, 5),
+                                                   (2, 300, 700, 8), (9, 16, 16, 5)])
+def test_batches_and_steps(dev, batch, rows, cols, steps):
+    r = np.random.default_rng(batch)
+    # scales far apart: every matrix is normalised by itself
+    x = np.stack([_gradient(r, rows, cols) * np.float32(10.0 ** (6 * i - 12)) for i in range(batch)])
+    x[-1] = _gradient(r, rows, cols)
+    got = dev.read(dev.orthogonalize(dev.upload(x), batch, rows, cols, steps)).reshape(x.shape)
+    for g, m in zip(got, x):
+        assert _rel(g, _orthogonalize(m, steps)) <= TOL
+
+
+@gpu
+def test_singular_values_are_driven_to_one(dev):
+    x = np.random.default_rng(5).standard_normal((96, 200)).astype(np.float32)
+    s = np.linalg.svd(dev.read(dev.orthogonalize(dev.upload(x), 1, 96, 200)).reshape(96, 200),
+                      compute_uv=False)
+    assert 0.6 < s.min() and s.max() < 1.25  # the quintic's range around 1
+
+
+@gpu
+def test_degenerate_inputs(dev):
+    run = lambda x: dev.read(dev.orthogonalize(dev.upload(x), 1, *x.shape)).reshape(x.shape)
+    np.testing.assert_array_equal(run(np.zeros((40, 70), np.float32)), np.zeros((40, 70)))
+    one = np.outer(np.arange(1, 41), np.linspace(-1, 1, 70)).astype(np.float32)  # rank 1
+    assert _rel(run(one), _orthogonalize(one)) <= DEGENERATE
+    tiny = np.random.default_rng(0).standard_normal((40, 70)).astype(np.float32) * np.float32(1e-30)
+    assert _rel(run(tiny), _orthogonalize(tiny)) <= TOL
+    big = np.random.default_rng(0).standard_normal((40, 70)).astype(np.float32) * np.float32(1e30)
+    assert _rel(run(big), _orthogonalize(big)) <= TOL
+    spike = np.zeros((70, 40), np.float32)
+    spike[3, 5] = -2.0  # one entry of size 1 after scaling
+    assert _rel(run(spike), _orthogonalize(spike)) <= DEGENERATE
+    bad = np.ones((40, 70), np.float32)
+    bad[1, 2] = np.nan
+    assert np.isnan(run(bad)).all()
+    assert dev.orthogonalize(dev.upload(np.zeros(0)), 0, 4, 4).len == 0
+    assert dev.orthogonalize(dev.upload(np.zeros(0)), 2, 0, 4).len == 0
+
+
+def _step(w, g, m, lr, mu, nesterov, wd, steps):
+    w, g, m = (a.astype(np.float64) for a in (w, g, m))
+    mu = float(np.float32(mu))
+    m = mu * m + (1 - mu) * g
+    u = (1 - mu) * g + mu * m if nesterov else m
+    gain = lr * 0.2 * np.sqrt(max(w.shape))
+    o = _orthogonalize(u, steps)
+    return (1 - lr * wd) * w - gain * o, m, gain * np.linalg.norm(o)
+
+
+@gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_optimizer_steps(dev, nesterov):
+    """Several steps over matrices of equal and different shapes in one call:
+    |W error| <= 4 u (|W| + |update|) + TOL |update| a step, momentum 4 u a step."""
+    from any_gpu import Muon
+    r = np.random.default_rng(7)
+    shapes = [(64, 96), (96, 64), (64, 96), (130, 33), (64, 64), (1, 50), (64, 96), (300, 260)]
+    opt = Muon(lr=0.05, nesterov=nesterov, weight_decay=0.1)
+    w = [r.standard_normal(s).astype(np.float32) for s in shapes]
+    params = [dev.upload(a) for a in w]
+    ref = [(a.astype(np.float64), np.zeros(a.shape)) for a in w]
+    err = np.zeros(len(w))
+    for step in range(3):
+        g = [_gradient(r, *s) for s in shapes]
+        opt.step(dev, params, [dev.upload(a) for a in g], shapes)
+        for i, (wi, mi) in enumerate(ref):
+            # each step from what the device holds, so errors do not add up
+            base = w[i] if step == 0 else held[i][0]
+            mom = mi if step == 0 else held[i][1]
+            want, m, size = _step(base, g[i], mom, 0.05, 0.95, nesterov, 0.1, 5)
+            got = dev.read(params[i]).reshape(want.shape)
+            got_m = dev.read(opt.states[i]).reshape(want.shape)
+            assert np.linalg.norm(got - want) <= (4 * U * (np.linalg.norm(want) + size)
+                                                  + TOL * size)
+            assert np.linalg.norm(got_m - m) <= 4 * U * (np.linalg.norm(m) + np.linalg.norm(g[i]))
+        held = [(dev.read(p).reshape(s), dev.read(m).reshape(s))
+                for p, m, s in zip(params, opt.states, shapes)]
+
+
+@gpu
+def test_caller_memory_unaligned_stream_and_graph(dev):
+    """Odd addresses, a caller's stream, and the same step replayed from two graphs."""
+    import torch
+    from any_gpu import muon_tensors
+    r = np.random.default_rng(2)
+    shapes = [(50, 77), (128, 128)]
+    start = [[_gradient(r, *s) for s in shapes] for _ in range(3)]
+    results = []
+    for mode in ("eager", "graph"):
+        hold = [[torch.cat([torch.zeros(1), torch.from_numpy(a).reshape(-1)]).cuda() for a in b]
+                for b in start]
+        ptr = lambda t: t.data_ptr() + 4
+        tensors = muon_tensors([(ptr(p), ptr(g), ptr(m), *s)
+                                for p, g, m, s in zip(*hold, shapes)])
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        call = lambda: dev.launch_muon(tensors, 0.02, 0.9, True, 0.0, 5, stream.cuda_stream)
+        if mode == "eager":
+            call()
+            call()
+        else:
+            graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+            for graph in graphs:
+                with torch.cuda.graph(graph, stream=stream):
+                    call()
+            with torch.cuda.stream(stream):
+                for graph in graphs:
+                    graph.replay()
+        torch.cuda.synchronize()
+        results.append(hold)
+        assert all(t[0] == 0 for b in hold for t in b)
+    for a, b in zip(*results):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    x = torch.from_numpy(start[0][0]).cuda()
+    torch.cuda.synchronize()
+    dev.launch_orthogonalize(x.data_ptr(), x.data_ptr(), 1, 50, 77)  # in place
+    dev.synchronize()
+    assert _rel(x.cpu().numpy(), _orthogonalize(start[0][0])) <= TOL
+
+
+@gpu
+def test_precision_mode_does_not_matter(dev):
+    x = dev.upload(_gradient(np.random.default_rng(0), 256, 384))
+    want = dev.read(dev.orthogonalize(x, 1, 256, 384))
+    for mode in ("tf32", "tf32x3", "ffma"):
+        with dev.precision(mode):
+            np.testing.assert_array_equal(dev.read(dev.orthogonalize(x, 1, 256, 384)), want)
+
+
+@gpu
+def test_buffer_layer_refusals(dev):
+    from any_gpu import AnyGpuError, Muon
+
+    def status(call):
+        with pytest.raises(AnyGpuError) as e:
+            call()
+        return e.value.status
+    x, y = dev.upload(np.ones(12)), dev.upload(np.ones(12))
+    assert status(lambda: dev.orthogonalize(x, 1, 3, 5)) == 1
+    assert status(lambda: dev.orthogonalize(x, 1, 3, 4, 0)) == 2
+    assert status(lambda: dev.orthogonalize(dev.upload_i32(np.ones(12, int)), 1, 3, 4)) == 2
+    assert status(lambda: Muon(0.1).step(dev, [x], [y], [(3, 5)])) == 1
+    assert status(lambda: Muon(0.1).step(dev, [x, x], [y, y], [(3, 4), (3, 4)])) == 2  # twice
+    assert status(lambda: Muon(0.1).step(dev, [x], [y, y], [(3, 4)])) == 1
+    np.testing.assert_array_equal(dev.read(x), np.ones(12))
+
+
+def test_launch_layer_refusals():
+    """Arguments are checked before the device: no GPU is needed to be refused."""
+    from any_gpu import _lib, muon_tensors
+    lib = _lib.load()
+    f, p = C.c_float, C.c_void_p(1 << 20)
+
+    def step(tensors=((1 << 20, 1 << 30, 1 << 24, 8, 8),), lr=0.1, mu=0.9, wd=0.0, steps=5):
+        t = muon_tensors(list(tensors))
+        return lib.agpu_launch_muon(None, C.addressof(t), len(t), f(lr), f(mu), 1, f(wd), steps,
+                                    None)
+    assert step(steps=0) == 2 and step(steps=65) == 2
+    assert step(mu=1.0) == 2 and step(mu=-0.1) == 2 and step(mu=float("nan")) == 2
+    assert step(lr=float("inf")) == 2 and step(wd=float("nan")) == 2
+    assert step(tensors=[(0, 1 << 30, 1 << 24, 8, 8)]) == 2
+    assert step(tensors=[(1 << 20, 0, 1 << 24, 8, 8)]) == 2
+    assert step(tensors=[(1 << 20, 1 << 30, 1 << 24, 2**31, 8)]) == 7
+    share = [(1 << 20, 1 << 30, 1 << 24, 8, 8), ((1 << 20) + 252, 1 << 30, 1 << 25, 8, 8)]
+    assert step(tensors=share) == 2 and b"share memory" in lib.agpu_last_error_message()
+    assert step(tensors=[(1 << 20, 1 << 30, 1 << 20, 8, 8)]) == 2  # momentum is the parameter
+    assert step() == 2 and b"NULL device" in lib.agpu_last_error_message()
+    orth = lambda *a: lib.agpu_launch_orthogonalize(None, *a, None)
+    assert orth(p, p, 1, 8, 8, 0) == 2
+    assert orth(None, p, 1, 8, 8, 5) == 2 and orth(p, None, 1, 8, 8, 5) == 2
+    assert orth(p, p, 1, 2**31, 1, 5) == 7
+    assert orth(p, p, 1, 8, 8, 5) == 2 and b"NULL device" in lib.agpu_last_error_message()
+
+
+def test_iteration_of_the_reference():
+    """The float64 iteration the GPU tests compare with, against its closed form on the
+    singular values."""
+    x = np.random.default_rng(1).standard_normal((6, 9))
+    u, s, vt = np.linalg.svd(x / np.linalg.norm(x), full_matrices=False)
+    for _ in range(5):
+        s = A * s + B * s ** 3 + CC * s ** 5
+    assert np.abs(_orthogonalize(x) - (u * s) @ vt).max() <= 1e-12
+    assert np.abs(_orthogonalize(x.T) - ((u * s) @ vt).T).max() <= 1e-12

@@ -4,23 +4,53 @@
 // matrices of a model.  For a matrix W with gradient G and momentum M:
 //   M <- mu M + (1 - mu) G,   U = (1 - mu) G + mu M (nesterov) or M
 //   X = U / max(|U|_F, 1e-30), then `steps` times (rows <= cols; else on X^T)
-//       A = X X^T,  X <- a X + (b A + c A A) X
+//       A = X X^T,  X <- (a I + b A + c A A) X
 //   W <- (1 - lr wd) W - lr 0.2 sqrt(max(rows, cols)) X
 // which drives the singular values of X towards 1.
+//
+// All matrices of a call go through the iteration together, a group per
+// launch: two kernels form the scaled split X, then three products a step
+// (muon_gemm.cuh), the last of which updates W in its epilogue.
 #include <algorithm>
 #include <cmath>
+#include <exception>
+#include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "agpu_internal.cuh"
+#include "muon_gemm.cuh"
 
 namespace agpu {
 
 namespace {
 
+using muon::Item;
+using muon::Mode;
+
 constexpr int kThreads = 256;
-constexpr int kParts = 1024;  // CTAs (and partial sums) of a norm
-constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr int kMaxParts = 1024;  // CTAs (and partial sums) of one matrix's norm
 constexpr double kNormFloor = 1e-30;
+constexpr size_t kGroupBytes = 8ull << 30;  // scratch of a group of several matrices
+constexpr int kGramRows = 512;  // least rows for steps on the Gram matrix
+
+// One matrix: what the call gives, and its scratch.
+struct Source {
+  const float* grad;
+  float* momentum;  // or null: the update is `grad`
+  __half* x;        // split X [m, n], two planes
+  long long plane;
+  int ld;           // of x: n rounded up to 64
+  int rows, cols;
+  int m, n;         // min, max
+};
+
+struct Sources {
+  Source item[muon::kMaxItems];
+  double* partial;  // [item][gridDim.x]
+  float mu;
+  int nesterov;
+};
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -35,129 +65,502 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return s;
 }
 
-// u = the update (momentum applied when there is one), and its squares' sums
+__device__ __forceinline__ float update_of(float g, float m, float mu, bool nesterov) {
+  return nesterov ? (1.0f - mu) * g + mu * m : m;
+}
+
+__device__ __forceinline__ float step_momentum(float g, float m, float mu) {
+  return mu * m + (1.0f - mu) * g;
+}
+
+__device__ __forceinline__ bool aligned16(const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+}
+
+// blockIdx.y = matrix.  Steps its momentum and sums the squares of its update
 // per CTA, in double: a gradient's squares leave the range of a float.
 __global__ void __launch_bounds__(kThreads)
-    muon_update_kernel(const float* __restrict__ grad, float* __restrict__ momentum,
-                       float* __restrict__ u, long long n, float mu, bool nesterov,
-                       double* __restrict__ partial) {
+    muon_update_kernel(const __grid_constant__ Sources p) {
   __shared__ double red[kThreads / 32];
+  const Source& it = p.item[blockIdx.y];
+  const long long n = (long long)it.rows * it.cols;
+  const bool vec = aligned16(it.grad) && aligned16(it.momentum);
   double s = 0.0;
-  for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < n;
-       i += (long long)gridDim.x * kThreads) {
-    float v = grad[i];
-    if (momentum) {
-      const float m = mu * momentum[i] + (1.0f - mu) * v;
-      momentum[i] = m;
-      v = nesterov ? (1.0f - mu) * v + mu * m : m;
+  for (long long i = (blockIdx.x * (long long)kThreads + threadIdx.x) * 4; i < n;
+       i += (long long)gridDim.x * kThreads * 4) {
+    float g[4], m[4];
+    const int cnt = (int)min(4ll, n - i);
+    if (vec && cnt == 4) {
+      *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(it.grad + i);
+      if (it.momentum)
+        *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(it.momentum + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[j] = j < cnt ? it.grad[i + j] : 0.f;
+        m[j] = j < cnt && it.momentum ? it.momentum[i + j] : 0.f;
+      }
     }
-    u[i] = v;
-    s += (double)v * v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float u = g[j];
+      if (it.momentum) {
+        m[j] = step_momentum(g[j], m[j], p.mu);
+        u = update_of(g[j], m[j], p.mu, p.nesterov);
+      }
+      s += (double)u * u;
+    }
+    if (it.momentum) {
+      if (vec && cnt == 4) {
+        *reinterpret_cast<float4*>(it.momentum + i) = *reinterpret_cast<float4*>(m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < cnt) it.momentum[i + j] = m[j];
+      }
+    }
   }
   s = block_sum(s, red);
-  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+  if (threadIdx.x == 0) p.partial[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
+// 8 scaled values to both planes, 16 bytes each.
+__device__ __forceinline__ void store_split(const float (&v)[8], __half* out, long long plane) {
+  auto pack = [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    *reinterpret_cast<uint4*>(out + P * plane) =
+        make_uint4(muon::pack2<P>(v[0], v[1]), muon::pack2<P>(v[2], v[3]),
+                   muon::pack2<P>(v[4], v[5]), muon::pack2<P>(v[6], v[7]));
+  };
+  pack(std::integral_constant<int, 0>());
+  pack(std::integral_constant<int, 1>());
+}
+
+// blockIdx.y = matrix.  X = its update over the norm, split, with rows along
+// the longer side (a tall matrix is transposed in shared memory); columns n to
+// ld are zero.
 __global__ void __launch_bounds__(kThreads)
-    muon_normalise_kernel(float* __restrict__ u, long long n, const double* __restrict__ partial,
-                          int parts) {
+    muon_split_kernel(const __grid_constant__ Sources p) {
   __shared__ double red[kThreads / 32];
+  __shared__ float tile[32][65];
+  const Source& it = p.item[blockIdx.y];
   double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kThreads) s += partial[i];
-  const float inv = (float)(1.0 / fmax(sqrt(block_sum(s, red)), kNormFloor));
-  for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < n;
-       i += (long long)gridDim.x * kThreads)
-    u[i] *= inv;
-}
-
-// y = p x + q y; y is only written when q is 0
-__global__ void __launch_bounds__(kThreads)
-    muon_axpby_kernel(const float* __restrict__ x, float* __restrict__ y, long long n, float p,
-                      float q) {
-  for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < n;
-       i += (long long)gridDim.x * kThreads)
-    y[i] = q != 0.0f ? p * x[i] + q * y[i] : p * x[i];
-}
-
-unsigned grid_for(long long n) {
-  return (unsigned)std::max<long long>(1, std::min<long long>((n + kThreads - 1) / kThreads,
-                                                              kParts));
-}
-
-struct PrecisionScope {
-  int saved;
-  explicit PrecisionScope(int mode) : saved(g_thread_precision) { g_thread_precision = mode; }
-  ~PrecisionScope() { g_thread_precision = saved; }
-};
-
-// X (scratch [rows, cols]) through the iteration; y, a, b are scratch.
-agpu_status iterate(agpu_device* dev, float*& x, float*& y, float* a, float* b, uint32_t rows,
-                    uint32_t cols, uint32_t steps, cudaStream_t s) {
-  const bool tall = rows > cols;
-  const uint32_t m = tall ? cols : rows, n = tall ? rows : cols;
-  const long long mm = (long long)m * m, mn = (long long)m * n;
-  PrecisionScope scope(AGPU_PREC_FFMA);
-  for (uint32_t i = 0; i < steps; ++i) {
-    AGPU_TRY(launch_gemm(dev, x, x, a, 1, m, m, n, tall, !tall, s));
-    AGPU_TRY(launch_gemm(dev, a, a, b, 1, m, m, m, false, false, s));
-    muon_axpby_kernel<<<grid_for(mm), kThreads, 0, s>>>(a, b, mm, kB, kC);
-    AGPU_TRY(after_launch(dev, "muon_axpby_kernel"));
-    if (tall) AGPU_TRY(launch_gemm(dev, x, b, y, 1, n, m, m, false, false, s));
-    else AGPU_TRY(launch_gemm(dev, b, x, y, 1, m, n, m, false, false, s));
-    muon_axpby_kernel<<<grid_for(mn), kThreads, 0, s>>>(x, y, mn, kA, 1.0f);
-    AGPU_TRY(after_launch(dev, "muon_axpby_kernel"));
-    std::swap(x, y);
+  for (int i = threadIdx.x; i < gridDim.x; i += kThreads)
+    s += p.partial[(long long)blockIdx.y * gridDim.x + i];
+  const double inv = muon::kXScale / fmax(sqrt(block_sum(s, red)), kNormFloor);
+  auto value = [&](long long i) {
+    const float g = it.grad[i];
+    return it.momentum ? update_of(g, it.momentum[i], p.mu, p.nesterov) : g;
+  };
+  if (it.rows <= it.cols) {
+    const int groups = it.ld / 8;
+    const long long total = (long long)it.m * groups;
+    const bool vec = it.cols % 4 == 0 && aligned16(it.grad) && aligned16(it.momentum);
+    for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < total;
+         i += (long long)gridDim.x * kThreads) {
+      const long long r = i / groups;
+      const int c = (int)(i - r * groups) * 8;
+      const long long at = r * it.cols + c;
+      float v[8];
+      if (vec && c + 8 <= it.cols) {
+        float m[8];
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          *reinterpret_cast<float4*>(v + h) = *reinterpret_cast<const float4*>(it.grad + at + h);
+          if (it.momentum)
+            *reinterpret_cast<float4*>(m + h) =
+                *reinterpret_cast<const float4*>(it.momentum + at + h);
+        }
+        if (it.momentum)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = update_of(v[j], m[j], p.mu, p.nesterov);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < it.cols ? value(at + j) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)(v[j] * inv);
+      store_split(v, it.x + r * it.ld + c, it.plane);
+    }
+    return;
   }
+  // tall: 64 source rows x 32 source columns -> 32 rows of 64
+  const int tiles_r = it.ld / 64, tiles_c = (it.cols + 31) / 32;
+  for (long long t = blockIdx.x; t < (long long)tiles_r * tiles_c; t += gridDim.x) {
+    const int r0 = (int)(t / tiles_c) * 64, c0 = (int)(t % tiles_c) * 32;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 32; i += kThreads) {
+      const int r = r0 + i / 32, c = c0 + i % 32;
+      tile[i % 32][i / 32] =
+          r < it.rows && c < it.cols ? (float)(value((long long)r * it.cols + c) * inv) : 0.f;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / 8, c = (threadIdx.x % 8) * 8;
+    if (c0 + r < it.m) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = tile[r][c + j];
+      store_split(v, it.x + (long long)(c0 + r) * it.ld + r0 + c, it.plane);
+    }
+  }
+}
+
+// ------------------------------------------------------ tensor-map encode --
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// A split matrix [rows, cols] of two planes.  k_major: tiles of 128 rows x 64
+// columns (the contraction runs along the rows' columns); else 64 rows (the
+// contraction) x 2 chunks of 64 columns.  A box holds both planes.
+agpu_status make_map(CUtensorMap* map, const __half* base, int rows, int cols, int ld,
+                     long long plane, bool k_major) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(AGPU_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t r = rows, c = cols, l = ld, pb = (cuuint64_t)plane * 2;
+  const cuuint64_t dk[3] = {c, r, 2}, sk[2] = {l * 2, pb};
+  const cuuint64_t dn[4] = {64, r, l / 64, 2}, sn[3] = {l * 2, 128, pb};
+  const cuuint32_t bk[3] = {64, 128, 2}, bn[4] = {64, 64, 2, 2}, es[4] = {1, 1, 1, 1};
+  const CUresult e =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, k_major ? 3 : 4, const_cast<__half*>(base),
+         k_major ? dk : dn, k_major ? sk : sn, k_major ? bk : bn, es,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e != CUDA_SUCCESS)
+    return fail(AGPU_ERR_CUDA, "orthogonalize: tensor map encode failed (%d)", (int)e);
   return AGPU_OK;
 }
 
-// out = decay * out + gain * (orthogonalised update)
-agpu_status update(agpu_device* dev, const float* grad, float* momentum, float* out, uint32_t rows,
-                   uint32_t cols, float mu, bool nesterov, float decay, float gain,
-                   uint32_t steps, cudaStream_t s) {
-  const long long n = (long long)rows * cols;
-  if (n == 0) return AGPU_OK;
-  const long long m = std::min(rows, cols);
+// ------------------------------------------------------------ the products --
+constexpr bool symmetric(Mode mode) { return mode != Mode::Step && mode != Mode::Update; }
+
+using Group = muon::Items<muon::kMaxItems>;
+
+template <bool PAIR, Mode MODE, int CAP>
+agpu_status launch_items(agpu_device* dev, const muon::Items<CAP>& g, cudaStream_t s) {
+  auto kern = muon::muon_gemm_kernel<PAIR, MODE, CAP>;
+  AGPU_CUDA((set_smem_once<muon::muon_gemm_kernel<PAIR, MODE, CAP>>(dev, muon::kSmem)));
+  const int slots = PAIR ? std::max(1, dev->sm_count / 2) : dev->sm_count;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min(g.tiles, slots) * (PAIR ? 2 : 1)), 1, 1);
+  cfg.blockDim = dim3(muon::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = muon::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  AGPU_CUDA(cudaLaunchKernelEx(&cfg, kern, g, dev->d_status));
+  return after_launch(dev, "muon_gemm_kernel");
+}
+
+// Tiles of a group's product with tiles of BN x BN.
+long long count_tiles(Mode mode, long long m, long long n, long long bn) {
+  const long long tm = (m + bn - 1) / bn, tn = (n + bn - 1) / bn;
+  return symmetric(mode) ? tm * (tm + 1) / 2 : tm * tn;
+}
+
+template <bool PAIR, Mode MODE>
+agpu_status launch_product(agpu_device* dev, Group& g, cudaStream_t s) {
+  constexpr int BN = PAIR ? 256 : 128;
+  long long tiles = 0;
+  for (int i = 0; i < g.count; ++i) {
+    Item& it = g.item[i];
+    it.tiles_m = (it.m + BN - 1) / BN;
+    it.tiles_n = (it.n + BN - 1) / BN;
+    it.first = (int)tiles;
+    tiles += count_tiles(MODE, it.m, it.n, BN);
+    if (tiles > 0x3fffffff) return fail(AGPU_ERR_UNSUPPORTED, "orthogonalize: too large");
+  }
+  g.tiles = (int)tiles;
+  if (g.count > muon::kFewItems)
+    return launch_items<PAIR, MODE, muon::kMaxItems>(dev, g, s);
+  muon::Items<muon::kFewItems> few;
+  std::copy(g.item, g.item + g.count, few.item);
+  few.count = g.count;
+  few.tiles = g.tiles;
+  return launch_items<PAIR, MODE, muon::kFewItems>(dev, few, s);
+}
+
+template <Mode MODE>
+agpu_status product(agpu_device* dev, Group& g, bool pair, cudaStream_t s) {
+  if (pair) return launch_product<true, MODE>(dev, g, s);
+  return launch_product<false, MODE>(dev, g, s);
+}
+
+// A symmetric [m, m] matrix, split; its tensor maps with K along the rows (k)
+// and across them (n).
+struct Square {
+  __half* p;
+  CUtensorMap k, n;
+};
+
+// One matrix through the iteration.
+struct Work {
+  Source src;
+  float* w;
+  float decay, gain;
+  __half* x[2];  // split X, in turn
+  CUtensorMap xk[2], xn[2];
+  Square sq[5];
+  int squares;       // of sq in use
+  long long square;  // elements of a plane of one
+  int ld_square;
+
+  size_t halves() const { return 4 * (size_t)src.plane + 2 * (size_t)squares * square; }
+};
+
+// Steps taken on the Gram matrix between two products with X.  With M =
+// a I + b A + c A A a step is X' = M X, so A' = X' X'^T = M A M: several steps
+// need X only at their ends, X' = (M_3 M_2 M_1) X, and products of [m, m]
+// matrices between, which commute and are symmetric.  In units of m^3 a step
+// on X costs 3 n/m + 1, a segment of three steps 3 n/m + 9 and of two
+// 3 n/m + 5: five steps as 3 + 2 take 6 n/m + 14 instead of 15 n/m + 5.
+// Rounding in A is amplified until the next X X^T, by up to 3.45^2 a step: in
+// fp32 arithmetic 3 + 2 stays within 1.5 times the error of single steps,
+// 5 in one segment is 10 to 100 times worse.
+constexpr int kMaxSegment = 3;
+
+// Length of segment i when `steps` are split into `segments`, longest first.
+int segment_length(int steps, int segments, int i) {
+  return steps / segments + (i < steps % segments ? 1 : 0);
+}
+
+agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float mu, bool nesterov,
+                      uint32_t steps, cudaStream_t s) {
+  size_t halves = 0;
+  long long most = 0, pairs = 0;
+  for (int i = 0; i < count; ++i) {
+    halves += w[i].halves();
+    most = std::max(most, (long long)w[i].src.rows * w[i].src.cols);
+    pairs += count_tiles(Mode::Gram, w[i].src.m, w[i].src.m, 256);
+  }
+  // pair tiles once the symmetric products fill the SMs with them; all
+  // products of a group alike, since the tile's size says which blocks of a
+  // symmetric matrix are stored
+  const bool pair = pairs >= dev->sm_count / 2;
+  const int parts = (int)std::max<long long>(1, std::min<long long>(kMaxParts, most / 4096));
   void* scratch = nullptr;
-  AGPU_TRY(pool_alloc(dev, kParts * sizeof(double) + (2 * n + 2 * m * m) * sizeof(float), &scratch,
-                      s));
-  double* partial = static_cast<double*>(scratch);
-  float* x = reinterpret_cast<float*>(partial + kParts);
-  float *a = x + n, *b = a + m * m, *y = b + m * m;
+  AGPU_TRY(pool_alloc(dev, halves * sizeof(__half) + (size_t)count * parts * sizeof(double),
+                      &scratch, s));
+  constexpr float X = muon::kXScale, M = muon::kMScale;
+  Group g = {};
+  // dst = scale * (a b) of every matrix's squares, added to g
+  auto add_mul = [&](int dst, int a, int b, float scale) {
+    for (int i = 0; i < count; ++i) {
+      Item& it = g.item[g.count++];
+      it.a = w[i].sq[a].k;
+      it.at = w[i].sq[a].n;
+      it.b = w[i].sq[b].k;
+      it.bt = w[i].sq[b].n;
+      it.m = it.n = it.k = w[i].src.m;
+      it.out = w[i].sq[dst].p;
+      it.plane = w[i].square;
+      it.ld = w[i].ld_square;
+      it.scale = scale;
+    }
+  };
   auto run = [&]() -> agpu_status {
-    const unsigned grid = grid_for(n);
-    muon_update_kernel<<<grid, kThreads, 0, s>>>(grad, momentum, x, n, mu, nesterov, partial);
+    Sources src = {};
+    src.mu = mu;
+    src.nesterov = nesterov;
+    __half* h = static_cast<__half*>(scratch);
+    for (int i = 0; i < count; ++i) {
+      Work& t = w[i];
+      const int m = t.src.m, n = t.src.n;
+      for (int k = 0; k < 2; ++k, h += 2 * t.src.plane) {
+        t.x[k] = h;
+        AGPU_TRY(make_map(&t.xk[k], h, m, n, t.src.ld, t.src.plane, true));
+        AGPU_TRY(make_map(&t.xn[k], h, m, n, t.src.ld, t.src.plane, false));
+      }
+      for (int k = 0; k < t.squares; ++k, h += 2 * t.square) {
+        t.sq[k].p = h;
+        AGPU_TRY(make_map(&t.sq[k].k, h, m, m, t.ld_square, t.square, true));
+        AGPU_TRY(make_map(&t.sq[k].n, h, m, m, t.ld_square, t.square, false));
+      }
+      t.src.x = t.x[0];
+      src.item[i] = t.src;
+    }
+    src.partial = reinterpret_cast<double*>(h);
+    const dim3 grid((unsigned)parts, (unsigned)count);
+    muon_update_kernel<<<grid, kThreads, 0, s>>>(src);
     AGPU_TRY(after_launch(dev, "muon_update_kernel"));
-    muon_normalise_kernel<<<grid, kThreads, 0, s>>>(x, n, partial, (int)grid);
-    AGPU_TRY(after_launch(dev, "muon_normalise_kernel"));
-    AGPU_TRY(iterate(dev, x, y, a, b, rows, cols, steps, s));
-    muon_axpby_kernel<<<grid, kThreads, 0, s>>>(x, out, n, gain, decay);
-    return after_launch(dev, "muon_axpby_kernel");
+    muon_split_kernel<<<grid, kThreads, 0, s>>>(src);
+    AGPU_TRY(after_launch(dev, "muon_split_kernel"));
+
+    const int segments =
+        on_gram ? ((int)steps + kMaxSegment - 1) / kMaxSegment : (int)steps;
+    for (int seg = 0; seg < segments; ++seg) {
+      const int len = segment_length((int)steps, segments, seg), cur = seg & 1;
+      // squares: A, the product of the segment's polynomials (in turn), the
+      // step's polynomial, and that times A
+      constexpr int kGram = 0, kPoly = 3, kPolyGram = 4;
+      int total = 1;
+      float total_scale = M;
+      g.count = count;
+      for (int i = 0; i < count; ++i) {  // A = X X^T
+        Item& it = g.item[i];
+        it.a = it.b = w[i].xk[cur];
+        it.m = it.n = w[i].src.m;
+        it.k = w[i].src.n;
+        it.out = w[i].sq[kGram].p;
+        it.plane = w[i].square;
+        it.ld = w[i].ld_square;
+        it.scale = 1.0f / X;
+      }
+      AGPU_TRY(product<Mode::Gram>(dev, g, pair, s));
+      for (int j = 0; j < len; ++j) {
+        const int poly = j ? kPoly : total;
+        g.count = 0;
+        add_mul(poly, kGram, kGram, muon::kC * (M / (X * X)));
+        for (int i = 0; i < count; ++i) g.item[i].g = w[i].sq[kGram].p;
+        AGPU_TRY(product<Mode::Poly>(dev, g, pair, s));
+        g.count = 0;
+        if (j + 1 < len) add_mul(kPolyGram, poly, kGram, 1.0f / M);
+        if (j) {
+          const float next = total_scale / 4;  // |polynomial| <= 3.45 a step
+          add_mul(3 - total, poly, total, next / (M * total_scale));
+          total = 3 - total;
+          total_scale = next;
+        }
+        if (g.count) AGPU_TRY(product<Mode::Mul>(dev, g, pair, s));
+        if (j + 1 < len) {  // A of the next step
+          g.count = 0;
+          add_mul(kGram, poly, kPolyGram, 1.0f / M);
+          AGPU_TRY(product<Mode::Mul>(dev, g, pair, s));
+        }
+      }
+      g.count = count;
+      for (int i = 0; i < count; ++i) {  // times X
+        Item& it = g.item[i];
+        it.a = w[i].sq[total].k;
+        it.at = w[i].sq[total].n;
+        it.bt = w[i].xn[cur];
+        it.m = it.k = w[i].src.m;
+        it.n = w[i].src.n;
+        it.out = w[i].x[1 - cur];
+        it.plane = w[i].src.plane;
+        it.ld = w[i].src.ld;
+        it.scale = 1.0f / total_scale;
+        it.w = w[i].w;
+        it.decay = w[i].decay;
+        it.gain = w[i].gain / (X * total_scale);
+        it.w_transposed = w[i].src.rows > w[i].src.cols;
+      }
+      if (seg + 1 < segments) AGPU_TRY(product<Mode::Step>(dev, g, pair, s));
+      else AGPU_TRY(product<Mode::Update>(dev, g, pair, s));
+    }
+    return AGPU_OK;
   };
   const agpu_status st = run();
   pool_free(dev, scratch, s);
   return st;
 }
 
+// Runs matrices of one kind in groups that fit a launch and the scratch limit.
+agpu_status run_groups(agpu_device* dev, std::vector<Work>& all, bool on_gram, float mu,
+                       bool nesterov, uint32_t steps, cudaStream_t s) {
+  const size_t most = on_gram ? muon::kMaxItems / 2 : muon::kMaxItems;
+  for (size_t first = 0; first < all.size();) {
+    size_t halves = all[first].halves(), end = first + 1;
+    while (end < all.size() && end - first < most &&
+           (halves + all[end].halves()) * sizeof(__half) <= kGroupBytes)
+      halves += all[end++].halves();
+    AGPU_TRY(run_group(dev, &all[first], (int)(end - first), on_gram, mu, nesterov, steps, s));
+    first = end;
+  }
+  return AGPU_OK;
+}
+
+// w = decay * w + gain * (orthogonalised update) of every matrix.
+agpu_status run_all(agpu_device* dev, std::vector<Work>& all, float mu, bool nesterov,
+                    uint32_t steps, cudaStream_t s) {
+  for (Work& t : all) {
+    Source& src = t.src;
+    src.m = std::min(src.rows, src.cols);
+    src.n = std::max(src.rows, src.cols);
+    if (src.n > 0x7fffff00) return fail(AGPU_ERR_UNSUPPORTED, "orthogonalize: too large");
+    src.ld = (src.n + 63) / 64 * 64;
+    src.plane = (long long)src.m * src.ld;
+    t.ld_square = (src.m + 63) / 64 * 64;
+    t.square = (long long)src.m * t.ld_square;
+    t.squares = 2;
+  }
+  // long contractions first, so that the last wave of a launch is short
+  std::stable_sort(all.begin(), all.end(), [](const Work& a, const Work& b) {
+    return a.src.m != b.src.m ? a.src.m > b.src.m : a.src.n > b.src.n;
+  });
+  // Steps on the Gram matrix for wide matrices, if there are enough of them
+  // to fill the SMs by themselves.
+  std::vector<Work> wide, rest;
+  long long pairs = 0;
+  for (const Work& t : all) {
+    const bool is_wide = steps > 1 && t.src.m >= kGramRows && t.src.n >= (3ll * t.src.m) / 2;
+    (is_wide ? wide : rest).push_back(t);
+    if (is_wide) pairs += count_tiles(Mode::Gram, t.src.m, t.src.m, 256);
+  }
+  if (pairs < dev->sm_count / 2) return run_groups(dev, all, false, mu, nesterov, steps, s);
+  for (Work& t : wide) t.squares = 5;
+  AGPU_TRY(run_groups(dev, wide, true, mu, nesterov, steps, s));
+  return run_groups(dev, rest, false, mu, nesterov, steps, s);
+}
+
 }  // namespace
 
 agpu_status launch_orthogonalize(agpu_device* dev, const float* x, float* out, uint32_t batch,
-                                 uint32_t rows, uint32_t cols, uint32_t steps, cudaStream_t s) {
+                                 uint32_t rows, uint32_t cols, uint32_t steps,
+                                 cudaStream_t s) try {
   const size_t n = (size_t)rows * cols;
-  for (uint32_t i = 0; i < batch; ++i)
-    AGPU_TRY(update(dev, x + i * n, nullptr, out + i * n, rows, cols, 0.f, false, 0.f, 1.f, steps,
-                    s));
-  return AGPU_OK;
+  if (n == 0) return AGPU_OK;
+  std::vector<Work> all(batch);
+  for (uint32_t i = 0; i < batch; ++i) {
+    all[i].src = {x + i * n, nullptr, nullptr, 0, 0, (int)rows, (int)cols, 0, 0};
+    all[i].w = out + i * n;
+    all[i].decay = 0.0f;
+    all[i].gain = 1.0f;
+  }
+  return run_all(dev, all, 0.0f, false, steps, s);
+} catch (const std::exception&) {
+  return fail(AGPU_ERR_OOM, "orthogonalize: out of host memory");
 }
 
 agpu_status launch_muon(agpu_device* dev, const agpu_muon_tensor* t, uint32_t count, float lr,
                         float momentum, bool nesterov, float weight_decay, uint32_t steps,
-                        cudaStream_t s) {
-  for (uint32_t i = 0; i < count; ++i)
-    AGPU_TRY(update(dev, t[i].grad, t[i].momentum, t[i].param, t[i].rows, t[i].cols, momentum,
-                    nesterov, 1.0f - lr * weight_decay,
-                    -lr * 0.2f * std::sqrt((float)std::max(t[i].rows, t[i].cols)), steps, s));
-  return AGPU_OK;
+                        cudaStream_t s) try {
+  std::vector<Work> all;
+  all.reserve(count);
+  for (uint32_t i = 0; i < count; ++i) {
+    if ((uint64_t)t[i].rows * t[i].cols == 0) continue;
+    Work w = {};
+    w.src = {t[i].grad, t[i].momentum, nullptr, 0, 0, (int)t[i].rows, (int)t[i].cols, 0, 0};
+    w.w = t[i].param;
+    w.decay = 1.0f - lr * weight_decay;
+    w.gain = -lr * 0.2f * std::sqrt((float)std::max(t[i].rows, t[i].cols));
+    all.push_back(w);
+  }
+  return run_all(dev, all, momentum, nesterov, steps, s);
+} catch (const std::exception&) {
+  return fail(AGPU_ERR_OOM, "muon_step: out of host memory");
 }
 
 }  // namespace agpu

@@ -1,0 +1,545 @@
+// The products of the Newton-Schulz iteration on tcgen05 (kind::f16), at
+// fp32-level accuracy, for a group of matrices of any shapes in one launch.
+//
+// Split operands.  Every matrix of the iteration is kept as two fp16 planes,
+// x 2^e = hi + lo with hi = fp16(x 2^e) and lo = fp16(x 2^e - hi): 22 bits of
+// each value in the 4 bytes a float takes.  The iteration bounds its values
+// (|X| <= 1.21, |A| <= 1.46, |a I + b A + c A A| <= 3.45 in the 2-norm, so
+// every entry too), and e is the power of two that brings this bound just
+// below fp16's largest value: the small entries of large matrices stay far
+// above fp16's subnormals.  A product is three MMAs into one fp32 accumulator,
+// lo hi + hi lo + hi hi (lo lo is below 2^-22), at the fp16 rate, twice
+// tf32's: half the time of the 3xTF32 GEMM (umma2_x3_kernel.cuh), which also
+// has to split its operands in a pass of its own.  Here the epilogue that
+// produces a matrix writes it split, so operands go from global memory
+// through TMA to the tensor core as they are.
+//
+// Segments.  The tensor core's fp32 sum truncates, an error that grows with
+// the number of MMAs summed (a K loop of 1024 in the 3xTF32 GEMM's segments of
+// 512 left 2.6e-5 after five steps, where fp32 FMAs leave 1e-6).  So an
+// accumulator takes K = 64 kSeg, small terms first, and the epilogue warps add
+// it, rounding to nearest, to a sum in registers while the tensor core fills
+// the other one.
+//
+// Symmetry.  A X X^T and products of commuting symmetric matrices are
+// symmetric: only tiles on and below the diagonal are computed and stored.
+// Whoever reads such a matrix takes a block above the diagonal from its mirror
+// image, as an MN-major operand instead of a K-major one (the descriptors and
+// the instruction's major bits change, the shared memory's size does not), so
+// nothing is stored twice.
+//
+// Tiles.  BN x BN outputs: 256 x 256 by a CTA pair (cta_group::2), or
+// 128 x 128 by one CTA for groups with few tiles.  Either way a stage holds, per
+// CTA, both planes of 128 rows of A and 128 of B by 64 of K: 64 KB, three
+// stages.
+//
+//   warp 0      TMA of the CTA's halves (no multicast)
+//   warp 1      tensor memory; one lane of the leader CTA issues the MMAs
+//   warps 4-11  epilogue: warp w owns 32 rows (w % 4) of half the columns, its
+//               sums in registers (128 of the 232 it takes over from warps 0-3)
+//
+// Every wait is bounded as in umma2_kernel.cuh.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace agpu {
+namespace muon {
+
+constexpr int kBK = 64;          // fp16 elements of K per stage: one 128-byte row
+constexpr int kSeg = 1;          // K-blocks summed by one accumulator
+constexpr int kStages = 3;
+constexpr int kEpi = 8;          // epilogue warps
+constexpr int kPlane = 128 * 128;          // bytes of one plane of an operand tile
+constexpr int kOperand = 2 * kPlane;       // hi and lo
+constexpr int kStage = 2 * kOperand;       // A and B
+constexpr int kStaging = 4096;             // bytes per epilogue warp
+constexpr int kSmem = 1024 + kStages * kStage + kEpi * kStaging + 256;
+constexpr int kThreads = 128 + 32 * kEpi;
+// Registers: 168 a thread at launch (384 threads), then 40 for warps 0-3 and
+// 232 for the epilogue: 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kRegsLow = 40, kRegsHigh = 232;
+// Matrices per launch.  They travel as kernel parameters, 640 bytes each;
+// launches of at most kFewItems keep below 4 KB.
+constexpr int kMaxItems = 24, kFewItems = 6;
+
+// Coefficients of the quintic and the exponents of the split matrices.
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr float kXScale = 32768.0f;  // X and A = X X^T
+constexpr float kMScale = 16384.0f;  // a I + b A + c A A
+
+// Operands and result of a product, with P = scale * (A B):
+enum class Mode {
+  Gram,   // A = B = X: out = P, symmetric
+  Poly,   // A = B symmetric: out = a I + b g + P, symmetric
+  Mul,    // A, B symmetric and commuting: out = P, symmetric
+  Step,   // A symmetric, B = X: out = P
+  Update  // A symmetric, B = X: w = decay * w + gain * (A B), fp32
+};
+
+struct Item {
+  // tiles of A and B with K along their rows, and across them (a block above
+  // the diagonal of a symmetric operand; X as B of Step and Update)
+  CUtensorMap a, at, b, bt;
+  int m, n, k;             // out [m, n], contraction k
+  int tiles_m, tiles_n, first;  // first: this item's first tile
+  __half* out;             // hi plane; the others follow, `plane` elements apart
+  const __half* g;         // split like out
+  long long plane;         // of out and g
+  int ld;                  // of out and g: a multiple of 64
+  float scale;
+  float* w;                // [m, n] or, if w_transposed, [n, m]
+  float decay, gain;
+  int w_transposed;
+};
+
+template <int CAP>
+struct Items {
+  Item item[CAP];
+  int count, tiles;
+};
+
+struct Tile {
+  int item, m0, n0;
+};
+
+template <bool SYM, int BN, int CAP>
+__device__ __forceinline__ Tile tile_at(const Items<CAP>& g, int t) {
+  Tile r;
+  r.item = 0;
+  while (r.item + 1 < g.count && t >= g.item[r.item + 1].first) ++r.item;
+  const Item& it = g.item[r.item];
+  const int q = t - it.first;
+  if (SYM) {
+    int i = (int)((sqrtf(8.0f * (float)q + 1.0f) - 1.0f) * 0.5f);
+    while (i * (i + 1) / 2 > q) --i;
+    while ((i + 1) * (i + 2) / 2 <= q) ++i;
+    r.m0 = i * BN;
+    r.n0 = (q - i * (i + 1) / 2) * BN;
+  } else {  // groups of 16 row tiles, rows fastest: B's column block stays in L2
+    constexpr int G = 16;
+    const int span = G * it.tiles_n;
+    const int first_m = (q / span) * G;
+    const int size = min(it.tiles_m - first_m, G);
+    r.m0 = (first_m + (q % span) % size) * BN;
+    r.n0 = ((q % span) / size) * BN;
+  }
+  return r;
+}
+
+// Plane P (0 = hi, 1 = lo, 2 = rest) of two scaled values, packed.
+template <int P>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  __half2 h = __floats2half2_rn(x, y);
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const float2 f = __half22float2(h);
+    x -= f.x;
+    y -= f.y;
+    h = __floats2half2_rn(x, y);
+  }
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// One plane of a warp's 32 x 64 block (thread = row) to global memory, through
+// 4 KB of shared memory in 16-byte pieces (XOR-swizzled: no bank conflicts).
+template <int P, int NC>
+__device__ __forceinline__ void store_block(const float (&v)[NC], int c0, uint8_t* stg, int lane,
+                                            __half* out, int ld, int rows) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 d;
+    d.x = pack2<P>(v[c0 + 8 * j + 0], v[c0 + 8 * j + 1]);
+    d.y = pack2<P>(v[c0 + 8 * j + 2], v[c0 + 8 * j + 3]);
+    d.z = pack2<P>(v[c0 + 8 * j + 4], v[c0 + 8 * j + 5]);
+    d.w = pack2<P>(v[c0 + 8 * j + 6], v[c0 + 8 * j + 7]);
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) * 16)) = d;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + lane / 8, j = lane % 8;
+    const uint4 d = *reinterpret_cast<uint4*>(stg + r * 128 + ((j ^ (r & 7)) * 16));
+    if (r < rows) *reinterpret_cast<uint4*>(out + (long long)r * ld + j * 8) = d;
+  }
+  __syncwarp();
+}
+
+// One plane of a 32 x 64 block of g, loaded by whole rows: issued ahead of its
+// use by add_block, which brings it to the threads' rows through shared memory.
+struct Block {
+  uint4 d[8];
+};
+
+__device__ __forceinline__ void load_block(Block& b, int lane, const __half* g, int ld,
+                                           int rows) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + lane / 8, j = lane % 8;
+    b.d[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows) b.d[i] = *reinterpret_cast<const uint4*>(g + (long long)r * ld + j * 8);
+  }
+}
+
+__device__ __forceinline__ void put_block(const Block& b, uint8_t* stg, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + lane / 8, j = lane % 8;
+    *reinterpret_cast<uint4*>(stg + r * 128 + ((j ^ (r & 7)) * 16)) = b.d[i];
+  }
+  __syncwarp();
+}
+
+// v += f * the block in shared memory.
+template <int NC>
+__device__ __forceinline__ void add_block(float (&v)[NC], int c0, float f, const uint8_t* stg,
+                                          int lane) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint4 d = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) * 16));
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[c0 + 8 * j + 2 * i] = fmaf(f, x.x, v[c0 + 8 * j + 2 * i]);
+      v[c0 + 8 * j + 2 * i + 1] = fmaf(f, x.y, v[c0 + 8 * j + 2 * i + 1]);
+    }
+  }
+  __syncwarp();
+}
+
+// w = decay w + gain v over a warp's 32 rows x NC columns of [m, n].
+template <int NC>
+__device__ __forceinline__ void update_block(const float (&v)[NC], uint8_t* stg, int lane,
+                                             float* w, bool transposed, float decay, float gain,
+                                             int m, int n, int row0, int col0) {
+  const bool keep = decay != 0.0f;  // 0: w is only written
+  if (transposed) {  // [n, m]: the warp's 32 rows are 32 neighbours in memory
+    const bool in = row0 + lane < m;
+    const int cols = n - col0;
+    w += (long long)col0 * m + row0 + lane;
+#pragma unroll
+    for (int c = 0; c < NC; c += 32) {
+      float old[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        old[j] = keep && in && c + j < cols ? w[(long long)(c + j) * m] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (in && c + j < cols)
+          w[(long long)(c + j) * m] = fmaf(gain, v[c + j], decay * old[j]);
+    }
+    return;
+  }
+  float* s = reinterpret_cast<float*>(stg);
+  const int rows = m - row0;
+  w += (long long)row0 * n + col0 + lane;
+#pragma unroll
+  for (int c = 0; c < NC; c += 32) {
+    const bool in = col0 + c + lane < n;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[lane * 32 + ((j + lane) & 31)] = v[c + j];
+    __syncwarp();
+    float old[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) old[r] = keep && in && r < rows ? w[(long long)r * n + c] : 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (in && r < rows)
+        w[(long long)r * n + c] = fmaf(gain, s[r * 32 + ((lane + r) & 31)], decay * old[r]);
+    __syncwarp();
+  }
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
+// a += b on two floats at once.
+__device__ __forceinline__ void add2(float& a0, float& a1, uint32_t b0, uint32_t b1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(b0), "r"(b1));
+}
+
+template <bool PAIR, Mode MODE, int CAP>
+__global__ void __launch_bounds__(kThreads, 1)
+    muon_gemm_kernel(const __grid_constant__ Items<CAP> g, unsigned int* status) {
+  constexpr bool SYM = MODE == Mode::Gram || MODE == Mode::Poly || MODE == Mode::Mul;
+  constexpr bool A_SYM = MODE != Mode::Gram;                       // A read by its lower tiles
+  constexpr bool B_SYM = MODE == Mode::Poly || MODE == Mode::Mul;  // B likewise
+  constexpr int BN = PAIR ? 256 : 128;   // tile rows and columns
+  constexpr int NC = BN / 2;             // columns of an epilogue warp
+  constexpr int CTAS = PAIR ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = ring + kStages * kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpi * kStaging);  // leader's is used
+  uint64_t* empty = full + kStages;    // both CTAs
+  uint64_t* tfull = empty + kStages;   // [2] both CTAs
+  uint64_t* tempty = tfull + 2;        // [2] leader's is used
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = PAIR ? (int)ptx::cluster_rank() : 0;
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&tfull[i], 1);
+      ptx::mbar_init(&tempty[i], CTAS * kEpi);  // one arrive per epilogue warp
+    }
+    ptx::mbar_init(drain, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      ptx::tmem_alloc_pair(tmem_slot, 2 * BN);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, 2 * BN);
+      ptx::tmem_relinquish();
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // peer barriers initialised, tensor memory allocated
+  ptx::tc_fence_after();
+  ptx::griddep_wait();  // the previous kernel's outputs are visible from here on
+  ptx::griddep_launch_dependents();
+  const uint32_t tmem_base = *tmem_slot;
+  const int cluster_id = blockIdx.x / CTAS, n_clusters = gridDim.x / CTAS;
+
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    const int q = warp & 3;                 // tensor-memory lanes 32 q ..
+    const int cbase = (warp - 4) / 4 * NC;  // columns of the tile
+    uint8_t* stg = staging + (warp - 4) * kStaging;
+    int unit = 0;
+    bool ok = true;
+    for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
+      const Tile tile = tile_at<SYM, BN, CAP>(g, t);
+      const Item& it = g.item[tile.item];
+      // copies: parameters indexed at run time would be fetched at every use
+      const int m = it.m, n = it.n, ld = it.ld;
+      const int num_k = (it.k + kBK - 1) / kBK;
+      const int row0 = tile.m0 + rank * 128 + q * 32, col0 = tile.n0 + cbase;
+      const bool live = row0 < m && col0 < n;
+      const long long plane = it.plane;
+      const long long at = (long long)row0 * ld + col0;
+      const __half* src = MODE == Mode::Poly ? it.g + at : nullptr;
+      if (MODE == Mode::Poly && row0 + lane < m) {
+#pragma unroll
+        for (int c = 0; c < NC; c += 64) {
+          if (col0 + c < n) {
+            prefetch_l2(src + (long long)lane * ld + c);
+            prefetch_l2(src + plane + (long long)lane * ld + c);
+          }
+        }
+      }
+      float v[NC];
+      Block next;  // the plane of g to be added next; the first before the last segment
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = 0.f;
+      for (int k0 = 0; k0 < num_k; k0 += kSeg, ++unit) {
+        const int acc = unit & 1;
+        if (MODE == Mode::Poly && live && k0 + kSeg >= num_k)
+          load_block(next, lane, src + plane, ld, m - row0);
+        // warp-uniform: every lane takes the same exit
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (unit >> 1) & 1, status, 0x605,
+                                                    abort_flag))) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t from = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + cbase;
+#pragma unroll
+        for (int c = 0; c < NC; c += 32) {
+          uint32_t x[32];
+          ptx::tmem_ld32(from + c, x);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) add2(v[c + i], v[c + i + 1], x[i], x[i + 1]);
+        }
+        // the accumulator is free again; the handoff carries no generic-memory
+        // data, so the peer's remote arrive is CTA-scope
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (leader) ptx::mbar_arrive(&tempty[acc]);
+          else ptx::mbar_arrive_remote(ptx::mapa(ptx::smem_u32(&tempty[acc]), 0));
+        }
+      }
+      if (!ok) break;
+      if (!live) continue;
+      if (MODE == Mode::Update) {
+        update_block<NC>(v, stg, lane, it.w, it.w_transposed, it.decay, it.gain, m, n, row0, col0);
+        continue;
+      }
+      const float scale = it.scale;
+      __half* out = it.out + at;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] *= scale;
+#pragma unroll
+      for (int c = 0; c < NC; c += 64) {
+        if (col0 + c >= n) break;
+        if (MODE == Mode::Poly) {  // small terms first
+          constexpr float f = kB * (kMScale / kXScale);
+          put_block(next, stg, lane);
+          load_block(next, lane, src + c, ld, m - row0);
+          add_block<NC>(v, c, f, stg, lane);
+          put_block(next, stg, lane);
+          if (c + 64 < NC && col0 + c + 64 < n)
+            load_block(next, lane, src + plane + c + 64, ld, m - row0);
+          add_block<NC>(v, c, f, stg, lane);
+          const int diagonal = row0 + lane - col0 - c;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i == diagonal) v[c + i] += kA * kMScale;
+        }
+        store_block<0, NC>(v, c, stg, lane, out + c, ld, m - row0);
+        store_block<1, NC>(v, c, stg, lane, out + plane + c, ld, m - row0);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    if (warp == 0) {
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        long long issued = 0;
+        for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
+          const Tile tile = tile_at<SYM, BN, CAP>(g, t);
+          const Item& it = g.item[tile.item];
+          const int num_k = (it.k + kBK - 1) / kBK;
+          const int am = tile.m0 + rank * 128, bn = tile.n0 + rank * 128;
+          for (int kb = 0; kb < num_k; ++kb) {
+            if (!ptx::mbar_wait(&empty[stage], phase ^ 1, status, 0x601, abort_flag)) {
+              ok = false;
+              break;
+            }
+            if (leader) ptx::mbar_arrive_expect_tx(&full[stage], CTAS * kStage);
+            uint8_t* sa = ring + stage * kStage;
+            uint8_t* sb = sa + kOperand;
+            const int k = kb * kBK;
+            const bool at = A_SYM && k >= tile.m0 + BN, bt = B_SYM ? k >= tile.n0 + BN : !SYM;
+            if (PAIR) {
+              const uint32_t bar = ptx::mapa(ptx::smem_u32(&full[stage]), 0);
+              if (at) ptx::tma_load_4d_pair(sa, &it.at, bar, 0, k, am / 64, 0);
+              else ptx::tma_load_3d_pair(sa, &it.a, bar, k, am, 0);
+              if (bt) ptx::tma_load_4d_pair(sb, &it.bt, bar, 0, k, bn / 64, 0);
+              else ptx::tma_load_3d_pair(sb, &it.b, bar, k, bn, 0);
+            } else {
+              if (at) ptx::tma_load_4d(sa, &it.at, &full[stage], 0, k, am / 64, 0);
+              else ptx::tma_load_3d(sa, &it.a, &full[stage], k, am, 0);
+              if (bt) ptx::tma_load_4d(sb, &it.bt, &full[stage], 0, k, bn / 64, 0);
+              else ptx::tma_load_3d(sb, &it.b, &full[stage], k, bn, 0);
+            }
+            ++issued;
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+          }
+        }
+        if (leader) {
+          // wait (bounded) for the last round of each stage, so that no copy of
+          // the CTAs is in flight when they exit
+          for (int s = 0; s < kStages && s < issued; ++s) {
+            const long long round = (issued - 1 - s) / kStages;
+            ptx::mbar_wait(&full[s], (uint32_t)(round & 1), status, 0x607, nullptr);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0 && leader) {
+        int stage = 0;
+        uint32_t phase = 0;
+        int unit = 0;  // segments so far
+        bool ok = true;
+        for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
+          const Tile tile = tile_at<SYM, BN, CAP>(g, t);
+          const int num_k = (g.item[tile.item].k + kBK - 1) / kBK;
+          for (int k0 = 0; k0 < num_k && ok; k0 += kSeg, ++unit) {
+            const int acc = unit & 1;
+            if (!ptx::mbar_wait<PAIR>(&tempty[acc], ((unit >> 1) & 1) ^ 1, status, 0x602,
+                                      abort_flag)) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            const uint32_t d = tmem_base + acc * BN;
+            const int k1 = min(num_k, k0 + kSeg);
+            for (int kb = k0; kb < k1; ++kb) {
+              if (!ptx::mbar_wait(&full[stage], phase, status, 0x603, abort_flag)) {
+                ok = false;
+                break;
+              }
+              ptx::tc_fence_after();
+              const uint32_t sa = ptx::smem_u32(ring + stage * kStage), sb = sa + kOperand;
+              const bool at = A_SYM && kb * kBK >= tile.m0 + BN;
+              const bool bt = B_SYM ? kb * kBK >= tile.n0 + BN : !SYM;
+              const uint32_t idesc =
+                  ptx::make_idesc_f16(CTAS * 128, BN, false, false) | (at << 15) | (bt << 16);
+              // K-major: 16 elements = 32 bytes along the swizzled row;
+              // MN-major: 16 rows of 128 bytes, 64-column chunks 8 KB apart
+              const uint64_t a0 = ptx::make_sdesc(sa, at ? 8192 : 16, 1024, 2);
+              const uint64_t b0 = ptx::make_sdesc(sb, bt ? 8192 : 16, 1024, 2);
+              const uint32_t a_step = at ? 2048 >> 4 : 32 >> 4, b_step = bt ? 2048 >> 4 : 32 >> 4;
+              auto a_desc = [&](int kk, int plane) {
+                return a0 + kk * a_step + plane * (kPlane >> 4);
+              };
+              auto b_desc = [&](int kk, int plane) {
+                return b0 + kk * b_step + plane * (kPlane >> 4);
+              };
+              auto mma = [&](uint64_t a, uint64_t b, bool more) {
+                if (PAIR) ptx::mma_f16_ss_pair(d, a, b, idesc, more);
+                else ptx::mma_f16_ss(d, a, b, idesc, more);
+              };
+  #pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk) {
+                mma(a_desc(kk, 1), b_desc(kk, 0), kb > k0 || kk > 0);
+                mma(a_desc(kk, 0), b_desc(kk, 1), true);
+              }
+  #pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk) mma(a_desc(kk, 0), b_desc(kk, 0), true);
+              if (PAIR) ptx::mma_commit_pair(&empty[stage], 0x3);
+              else ptx::mma_commit(&empty[stage]);
+              if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            if (PAIR) ptx::mma_commit_pair(&tfull[acc], 0x3);
+            else ptx::mma_commit(&tfull[acc]);
+          }
+        }
+        if (PAIR) ptx::mma_commit_pair(drain, 0x3);
+        else ptx::mma_commit(drain);
+        ptx::mbar_wait(drain, 0, status, 0x604, nullptr);
+      }
+    }
+  }
+
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // the pair's MMAs are retired before either frees TMEM
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    if (PAIR) ptx::tmem_dealloc_pair(tmem_base, 2 * BN);
+    else ptx::tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+}  // namespace muon
+}  // namespace agpu

@@ -15,7 +15,6 @@
 #include <cmath>
 #include <exception>
 #include <mutex>
-#include <type_traits>
 #include <vector>
 
 #include "agpu_internal.cuh"
@@ -126,14 +125,13 @@ __global__ void __launch_bounds__(kThreads)
 
 // 8 scaled values to both planes, 16 bytes each.
 __device__ __forceinline__ void store_split(const float (&v)[8], __half* out, long long plane) {
-  auto pack = [&](auto p) {
-    constexpr int P = decltype(p)::value;
-    *reinterpret_cast<uint4*>(out + P * plane) =
-        make_uint4(muon::pack2<P>(v[0], v[1]), muon::pack2<P>(v[2], v[3]),
-                   muon::pack2<P>(v[4], v[5]), muon::pack2<P>(v[6], v[7]));
-  };
-  pack(std::integral_constant<int, 0>());
-  pack(std::integral_constant<int, 1>());
+  uint4 hi, lo;
+  muon::split2(v[0], v[1], hi.x, lo.x);
+  muon::split2(v[2], v[3], hi.y, lo.y);
+  muon::split2(v[4], v[5], hi.z, lo.z);
+  muon::split2(v[6], v[7], hi.w, lo.w);
+  *reinterpret_cast<uint4*>(out) = hi;
+  *reinterpret_cast<uint4*>(out + plane) = lo;
 }
 
 // blockIdx.y = matrix.  X = its update over the norm, split, with rows along
@@ -144,6 +142,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ double red[kThreads / 32];
   __shared__ float tile[32][65];
   const Source& it = p.item[blockIdx.y];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   double s = 0.0;
   for (int i = threadIdx.x; i < gridDim.x; i += kThreads)
     s += p.partial[(long long)blockIdx.y * gridDim.x + i];
@@ -189,11 +188,14 @@ __global__ void __launch_bounds__(kThreads)
   for (long long t = blockIdx.x; t < (long long)tiles_r * tiles_c; t += gridDim.x) {
     const int r0 = (int)(t / tiles_c) * 64, c0 = (int)(t % tiles_c) * 32;
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 32; i += kThreads) {
-      const int r = r0 + i / 32, c = c0 + i % 32;
-      tile[i % 32][i / 32] =
-          r < it.rows && c < it.cols ? (float)(value((long long)r * it.cols + c) * inv) : 0.f;
+    float u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = r0 + warp + 8 * j, c = c0 + lane;
+      u[j] = r < it.rows && c < it.cols ? value((long long)r * it.cols + c) : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tile[lane][warp + 8 * j] = (float)(u[j] * inv);
     __syncthreads();
     const int r = threadIdx.x / 8, c = (threadIdx.x % 8) * 8;
     if (c0 + r < it.m) {
@@ -247,14 +249,12 @@ agpu_status make_map(CUtensorMap* map, const __half* base, int rows, int cols, i
 }
 
 // ------------------------------------------------------------ the products --
-constexpr bool symmetric(Mode mode) { return mode != Mode::Step && mode != Mode::Update; }
-
 using Group = muon::Items<muon::kMaxItems>;
 
-template <bool PAIR, Mode MODE, int CAP>
+template <bool PAIR, int CAP>
 agpu_status launch_items(agpu_device* dev, const muon::Items<CAP>& g, cudaStream_t s) {
-  auto kern = muon::muon_gemm_kernel<PAIR, MODE, CAP>;
-  AGPU_CUDA((set_smem_once<muon::muon_gemm_kernel<PAIR, MODE, CAP>>(dev, muon::kSmem)));
+  auto kern = muon::muon_gemm_kernel<PAIR, CAP>;
+  AGPU_CUDA((set_smem_once<muon::muon_gemm_kernel<PAIR, CAP>>(dev, muon::kSmem)));
   const int slots = PAIR ? std::max(1, dev->sm_count / 2) : dev->sm_count;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(std::min(g.tiles, slots) * (PAIR ? 2 : 1)), 1, 1);
@@ -274,13 +274,15 @@ agpu_status launch_items(agpu_device* dev, const muon::Items<CAP>& g, cudaStream
   return after_launch(dev, "muon_gemm_kernel");
 }
 
-// Tiles of a group's product with tiles of BN x BN.
+// Tiles of one matrix's product with tiles of bn x bn.
 long long count_tiles(Mode mode, long long m, long long n, long long bn) {
   const long long tm = (m + bn - 1) / bn, tn = (n + bn - 1) / bn;
-  return symmetric(mode) ? tm * (tm + 1) / 2 : tm * tn;
+  if (!muon::symmetric_out(mode)) return tm * tn;
+  const long long blocks = (m + muon::kBlock - 1) / muon::kBlock, sub = muon::kBlock / bn;
+  return blocks * (blocks + 1) / 2 * sub * sub;
 }
 
-template <bool PAIR, Mode MODE>
+template <bool PAIR>
 agpu_status launch_product(agpu_device* dev, Group& g, cudaStream_t s) {
   constexpr int BN = PAIR ? 256 : 128;
   long long tiles = 0;
@@ -289,23 +291,35 @@ agpu_status launch_product(agpu_device* dev, Group& g, cudaStream_t s) {
     it.tiles_m = (it.m + BN - 1) / BN;
     it.tiles_n = (it.n + BN - 1) / BN;
     it.first = (int)tiles;
-    tiles += count_tiles(MODE, it.m, it.n, BN);
+    tiles += count_tiles(g.mode, it.m, it.n, BN);
     if (tiles > 0x3fffffff) return fail(AGPU_ERR_UNSUPPORTED, "orthogonalize: too large");
   }
   g.tiles = (int)tiles;
   if (g.count > muon::kFewItems)
-    return launch_items<PAIR, MODE, muon::kMaxItems>(dev, g, s);
+    return launch_items<PAIR, muon::kMaxItems>(dev, g, s);
   muon::Items<muon::kFewItems> few;
   std::copy(g.item, g.item + g.count, few.item);
   few.count = g.count;
   few.tiles = g.tiles;
-  return launch_items<PAIR, MODE, muon::kFewItems>(dev, few, s);
+  few.mode = g.mode;
+  return launch_items<PAIR, muon::kFewItems>(dev, few, s);
 }
 
-template <Mode MODE>
-agpu_status product(agpu_device* dev, Group& g, bool pair, cudaStream_t s) {
-  if (pair) return launch_product<true, MODE>(dev, g, s);
-  return launch_product<false, MODE>(dev, g, s);
+// Pair tiles (4 times the work on twice the SMs) once their waves are worth it:
+// a wave of them took 20 us where one of single tiles took 15 (products with X of
+// eight matrices around 1024 x 2816, K = 1024).
+agpu_status product(agpu_device* dev, Mode mode, Group& g, cudaStream_t s) {
+  g.mode = mode;
+  long long pairs = 0, singles = 0;
+  for (int i = 0; i < g.count; ++i) {
+    pairs += count_tiles(mode, g.item[i].m, g.item[i].n, 256);
+    singles += count_tiles(mode, g.item[i].m, g.item[i].n, 128);
+  }
+  const long long sms = dev->sm_count;
+  const long long pair_waves = ceil_div(pairs, std::max(1ll, sms / 2));
+  if (4 * pair_waves <= 3 * (long long)ceil_div(singles, sms))
+    return launch_product<true>(dev, g, s);
+  return launch_product<false>(dev, g, s);
 }
 
 // A symmetric [m, m] matrix, split; its tensor maps with K along the rows (k)
@@ -349,16 +363,11 @@ int segment_length(int steps, int segments, int i) {
 agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float mu, bool nesterov,
                       uint32_t steps, cudaStream_t s) {
   size_t halves = 0;
-  long long most = 0, pairs = 0;
+  long long most = 0;
   for (int i = 0; i < count; ++i) {
     halves += w[i].halves();
     most = std::max(most, (long long)w[i].src.rows * w[i].src.cols);
-    pairs += count_tiles(Mode::Gram, w[i].src.m, w[i].src.m, 256);
   }
-  // pair tiles once the symmetric products fill the SMs with them; all
-  // products of a group alike, since the tile's size says which blocks of a
-  // symmetric matrix are stored
-  const bool pair = pairs >= dev->sm_count / 2;
   const int parts = (int)std::max<long long>(1, std::min<long long>(kMaxParts, most / 4096));
   void* scratch = nullptr;
   AGPU_TRY(pool_alloc(dev, halves * sizeof(__half) + (size_t)count * parts * sizeof(double),
@@ -428,13 +437,13 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
         it.ld = w[i].ld_square;
         it.scale = 1.0f / X;
       }
-      AGPU_TRY(product<Mode::Gram>(dev, g, pair, s));
+      AGPU_TRY(product(dev, Mode::Gram, g, s));
       for (int j = 0; j < len; ++j) {
         const int poly = j ? kPoly : total;
         g.count = 0;
         add_mul(poly, kGram, kGram, muon::kC * (M / (X * X)));
         for (int i = 0; i < count; ++i) g.item[i].g = w[i].sq[kGram].p;
-        AGPU_TRY(product<Mode::Poly>(dev, g, pair, s));
+        AGPU_TRY(product(dev, Mode::Poly, g, s));
         g.count = 0;
         if (j + 1 < len) add_mul(kPolyGram, poly, kGram, 1.0f / M);
         if (j) {
@@ -443,11 +452,11 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
           total = 3 - total;
           total_scale = next;
         }
-        if (g.count) AGPU_TRY(product<Mode::Mul>(dev, g, pair, s));
+        if (g.count) AGPU_TRY(product(dev, Mode::Mul, g, s));
         if (j + 1 < len) {  // A of the next step
           g.count = 0;
           add_mul(kGram, poly, kPolyGram, 1.0f / M);
-          AGPU_TRY(product<Mode::Mul>(dev, g, pair, s));
+          AGPU_TRY(product(dev, Mode::Mul, g, s));
         }
       }
       g.count = count;
@@ -467,8 +476,8 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
         it.gain = w[i].gain / (X * total_scale);
         it.w_transposed = w[i].src.rows > w[i].src.cols;
       }
-      if (seg + 1 < segments) AGPU_TRY(product<Mode::Step>(dev, g, pair, s));
-      else AGPU_TRY(product<Mode::Update>(dev, g, pair, s));
+      if (seg + 1 < segments) AGPU_TRY(product(dev, Mode::Step, g, s));
+      else AGPU_TRY(product(dev, Mode::Update, g, s));
     }
     return AGPU_OK;
   };

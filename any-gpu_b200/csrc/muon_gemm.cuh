@@ -22,14 +22,14 @@
 // the other one.
 //
 // Symmetry.  A X X^T and products of commuting symmetric matrices are
-// symmetric: only tiles on and below the diagonal are computed and stored.
-// Whoever reads such a matrix takes a block above the diagonal from its mirror
+// symmetric: only 256 x 256 blocks on and below the diagonal are computed and
+// stored.  Whoever reads such a matrix takes a block above the diagonal from its mirror
 // image, as an MN-major operand instead of a K-major one (the descriptors and
 // the instruction's major bits change, the shared memory's size does not), so
 // nothing is stored twice.
 //
 // Tiles.  BN x BN outputs: 256 x 256 by a CTA pair (cta_group::2), or
-// 128 x 128 by one CTA for groups with few tiles.  Either way a stage holds, per
+// 128 x 128 by one CTA for products with few tiles.  Either way a stage holds, per
 // CTA, both planes of 128 rows of A and 128 of B by 64 of K: 64 KB, three
 // stages.
 //
@@ -49,6 +49,7 @@
 namespace agpu {
 namespace muon {
 
+constexpr int kBlock = 256;      // blocks of a symmetric matrix: whole ones are stored
 constexpr int kBK = 64;          // fp16 elements of K per stage: one 128-byte row
 constexpr int kSeg = 1;          // K-blocks summed by one accumulator
 constexpr int kStages = 3;
@@ -100,25 +101,32 @@ template <int CAP>
 struct Items {
   Item item[CAP];
   int count, tiles;
+  Mode mode;
 };
+
+__host__ __device__ constexpr bool symmetric_out(Mode m) {
+  return m == Mode::Gram || m == Mode::Poly || m == Mode::Mul;
+}
 
 struct Tile {
   int item, m0, n0;
 };
 
-template <bool SYM, int BN, int CAP>
+template <int BN, int CAP>
 __device__ __forceinline__ Tile tile_at(const Items<CAP>& g, int t) {
   Tile r;
   r.item = 0;
   while (r.item + 1 < g.count && t >= g.item[r.item + 1].first) ++r.item;
   const Item& it = g.item[r.item];
   const int q = t - it.first;
-  if (SYM) {
-    int i = (int)((sqrtf(8.0f * (float)q + 1.0f) - 1.0f) * 0.5f);
-    while (i * (i + 1) / 2 > q) --i;
-    while ((i + 1) * (i + 2) / 2 <= q) ++i;
-    r.m0 = i * BN;
-    r.n0 = (q - i * (i + 1) / 2) * BN;
+  if (symmetric_out(g.mode)) {  // blocks of the lower triangle by rows, (kBlock / BN)^2 tiles each
+    constexpr int S = kBlock / BN;
+    const int blk = q / (S * S), sub = q % (S * S);
+    int i = (int)((sqrtf(8.0f * (float)blk + 1.0f) - 1.0f) * 0.5f);
+    while (i * (i + 1) / 2 > blk) --i;
+    while ((i + 1) * (i + 2) / 2 <= blk) ++i;
+    r.m0 = i * kBlock + sub / S * BN;
+    r.n0 = (blk - i * (i + 1) / 2) * kBlock + sub % S * BN;
   } else {  // groups of 16 row tiles, rows fastest: B's column block stays in L2
     constexpr int G = 16;
     const int span = G * it.tiles_n;
@@ -130,128 +138,144 @@ __device__ __forceinline__ Tile tile_at(const Items<CAP>& g, int t) {
   return r;
 }
 
-// Plane P (0 = hi, 1 = lo, 2 = rest) of two scaled values, packed.
-template <int P>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  __half2 h = __floats2half2_rn(x, y);
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const float2 f = __half22float2(h);
-    x -= f.x;
-    y -= f.y;
-    h = __floats2half2_rn(x, y);
-  }
-  return *reinterpret_cast<uint32_t*>(&h);
+// K-blocks of a tile (none outside the matrix: a part of a diagonal block).
+__device__ __forceinline__ int k_blocks(const Item& it, const Tile& t) {
+  return t.m0 < it.m && t.n0 < it.n ? (it.k + kBK - 1) / kBK : 0;
 }
 
-// One plane of a warp's 32 x 64 block (thread = row) to global memory, through
-// 4 KB of shared memory in 16-byte pieces (XOR-swizzled: no bank conflicts).
-template <int P, int NC>
-__device__ __forceinline__ void store_block(const float (&v)[NC], int c0, uint8_t* stg, int lane,
+// hi and lo of two scaled values, packed.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// The epilogue takes a warp's 32 rows in blocks of 64 columns, the next one
+// always in v[0..63]: a loop, not code unrolled over all 128 columns, and one
+// kernel for all modes.  A tile's 128 KB per CTA leave in 5,500 cycles when all
+// CTAs store at once (3.4 KB a cycle, what L2 takes); with a kernel per mode and
+// unrolled code the first tile of a launch took 13,000, waiting for
+// instructions, and blocks of 32 columns (64-byte runs) 11,000.
+//
+// A plane of a block passes through 4 KB of shared memory per warp, a 128-byte
+// line per row in 16-byte pieces, piece j of line r at j ^ (r % 8), so that
+// neither rows nor lines conflict on banks.
+__device__ __forceinline__ uint8_t* piece(uint8_t* stg, int line, int j) {
+  return stg + line * 128 + ((j ^ (line & 7)) << 4);
+}
+
+// One plane of a block, a row per thread, to global memory by lines.
+__device__ __forceinline__ void store_plane(const uint32_t (&h)[32], uint8_t* stg, int lane,
                                             __half* out, int ld, int rows) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint4 d;
-    d.x = pack2<P>(v[c0 + 8 * j + 0], v[c0 + 8 * j + 1]);
-    d.y = pack2<P>(v[c0 + 8 * j + 2], v[c0 + 8 * j + 3]);
-    d.z = pack2<P>(v[c0 + 8 * j + 4], v[c0 + 8 * j + 5]);
-    d.w = pack2<P>(v[c0 + 8 * j + 6], v[c0 + 8 * j + 7]);
-    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) * 16)) = d;
-  }
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(piece(stg, lane, j)) =
+        make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
   __syncwarp();
+  out += (long long)(lane >> 3) * ld + (lane & 7) * 8;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + lane / 8, j = lane % 8;
-    const uint4 d = *reinterpret_cast<uint4*>(stg + r * 128 + ((j ^ (r & 7)) * 16));
-    if (r < rows) *reinterpret_cast<uint4*>(out + (long long)r * ld + j * 8) = d;
+    const int line = i * 4 + (lane >> 3);
+    const uint4 d = *reinterpret_cast<uint4*>(piece(stg, line, lane & 7));
+    if (line < rows) *reinterpret_cast<uint4*>(out + (long long)i * 4 * ld) = d;
   }
   __syncwarp();
 }
 
-// One plane of a 32 x 64 block of g, loaded by whole rows: issued ahead of its
-// use by add_block, which brings it to the threads' rows through shared memory.
+// One plane of a block of g, loaded by lines ahead of its use (lines behind the
+// last row repeat it: their sums are not stored).
 struct Block {
   uint4 d[8];
 };
 
 __device__ __forceinline__ void load_block(Block& b, int lane, const __half* g, int ld,
                                            int rows) {
+  g += (long long)(lane >> 3) * ld + (lane & 7) * 8;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + lane / 8, j = lane % 8;
     b.d[i] = make_uint4(0, 0, 0, 0);
-    if (r < rows) b.d[i] = *reinterpret_cast<const uint4*>(g + (long long)r * ld + j * 8);
+    if (i * 4 + (lane >> 3) < rows)
+      b.d[i] = *reinterpret_cast<const uint4*>(g + (long long)i * 4 * ld);
   }
 }
 
 __device__ __forceinline__ void put_block(const Block& b, uint8_t* stg, int lane) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + lane / 8, j = lane % 8;
-    *reinterpret_cast<uint4*>(stg + r * 128 + ((j ^ (r & 7)) * 16)) = b.d[i];
-  }
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<uint4*>(piece(stg, i * 4 + (lane >> 3), lane & 7)) = b.d[i];
   __syncwarp();
 }
 
-// v += f * the block in shared memory.
-template <int NC>
-__device__ __forceinline__ void add_block(float (&v)[NC], int c0, float f, const uint8_t* stg,
-                                          int lane) {
+// v += f * the staged block.
+__device__ __forceinline__ void add_block(float* v, float f, uint8_t* stg, int lane) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const uint4 d = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) * 16));
+    const uint4 d = *reinterpret_cast<const uint4*>(piece(stg, lane, j));
     const uint32_t w[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[c0 + 8 * j + 2 * i] = fmaf(f, x.x, v[c0 + 8 * j + 2 * i]);
-      v[c0 + 8 * j + 2 * i + 1] = fmaf(f, x.y, v[c0 + 8 * j + 2 * i + 1]);
+      v[8 * j + 2 * i] = fmaf(f, x.x, v[8 * j + 2 * i]);
+      v[8 * j + 2 * i + 1] = fmaf(f, x.y, v[8 * j + 2 * i + 1]);
     }
   }
   __syncwarp();
 }
 
-// w = decay w + gain v over a warp's 32 rows x NC columns of [m, n].
-template <int NC>
-__device__ __forceinline__ void update_block(const float (&v)[NC], uint8_t* stg, int lane,
-                                             float* w, bool transposed, float decay, float gain,
-                                             int m, int n, int row0, int col0) {
+// w = decay w + gain v for 32 x 32 values, `rows` x `cols` of them inside the
+// matrix, w at the first; through shared memory, so that global memory is
+// accessed along its lines whether w is stored like v or transposed.
+__device__ __forceinline__ void update_block(const float* v, uint8_t* stg, int lane, float* w,
+                                             long long pitch, bool transposed, float decay,
+                                             float gain, int rows, int cols) {
   const bool keep = decay != 0.0f;  // 0: w is only written
-  if (transposed) {  // [n, m]: the warp's 32 rows are 32 neighbours in memory
-    const bool in = row0 + lane < m;
-    const int cols = n - col0;
-    w += (long long)col0 * m + row0 + lane;
+  if (transposed) {
 #pragma unroll
-    for (int c = 0; c < NC; c += 32) {
-      float old[32];
+    for (int j = 0; j < 32; ++j)
+      *reinterpret_cast<float*>(piece(stg, j, lane >> 2) + (lane & 3) * 4) = v[j];
+  } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        old[j] = keep && in && c + j < cols ? w[(long long)(c + j) * m] : 0.f;
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float4*>(piece(stg, lane, j)) =
+          make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+  __syncwarp();
+  const int lines = transposed ? cols : rows, len = transposed ? rows : cols;
+  if (pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && len >= 32) {
+    const int l0 = lane >> 3, p = lane & 7;
+    float4 old[8];
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (in && c + j < cols)
-          w[(long long)(c + j) * m] = fmaf(gain, v[c + j], decay * old[j]);
+    for (int i = 0; i < 8; ++i) {
+      old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (keep && i * 4 + l0 < lines)
+        old[i] = *reinterpret_cast<const float4*>(w + (i * 4 + l0) * pitch + p * 4);
     }
-    return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int l = i * 4 + l0;
+      const float4 x = *reinterpret_cast<const float4*>(piece(stg, l, p));
+      if (l < lines)
+        *reinterpret_cast<float4*>(w + l * pitch + p * 4) =
+            make_float4(fmaf(gain, x.x, decay * old[i].x), fmaf(gain, x.y, decay * old[i].y),
+                        fmaf(gain, x.z, decay * old[i].z), fmaf(gain, x.w, decay * old[i].w));
+    }
+  } else {
+    for (int l0 = 0; l0 < 32; l0 += 8) {
+      float old[8];
+#pragma unroll
+      for (int l = 0; l < 8; ++l)
+        old[l] = keep && l0 + l < lines && lane < len ? w[(l0 + l) * pitch + lane] : 0.f;
+#pragma unroll
+      for (int l = 0; l < 8; ++l) {
+        const float x = *reinterpret_cast<float*>(piece(stg, l0 + l, lane >> 2) + (lane & 3) * 4);
+        if (l0 + l < lines && lane < len)
+          w[(l0 + l) * pitch + lane] = fmaf(gain, x, decay * old[l]);
+      }
+    }
   }
-  float* s = reinterpret_cast<float*>(stg);
-  const int rows = m - row0;
-  w += (long long)row0 * n + col0 + lane;
-#pragma unroll
-  for (int c = 0; c < NC; c += 32) {
-    const bool in = col0 + c + lane < n;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) s[lane * 32 + ((j + lane) & 31)] = v[c + j];
-    __syncwarp();
-    float old[32];
-#pragma unroll
-    for (int r = 0; r < 32; ++r) old[r] = keep && in && r < rows ? w[(long long)r * n + c] : 0.f;
-#pragma unroll
-    for (int r = 0; r < 32; ++r)
-      if (in && r < rows)
-        w[(long long)r * n + c] = fmaf(gain, s[r * 32 + ((lane + r) & 31)], decay * old[r]);
-    __syncwarp();
-  }
+  __syncwarp();
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -267,12 +291,14 @@ __device__ __forceinline__ void add2(float& a0, float& a1, uint32_t b0, uint32_t
       : "r"(b0), "r"(b1));
 }
 
-template <bool PAIR, Mode MODE, int CAP>
+template <bool PAIR, int CAP>
 __global__ void __launch_bounds__(kThreads, 1)
     muon_gemm_kernel(const __grid_constant__ Items<CAP> g, unsigned int* status) {
-  constexpr bool SYM = MODE == Mode::Gram || MODE == Mode::Poly || MODE == Mode::Mul;
-  constexpr bool A_SYM = MODE != Mode::Gram;                       // A read by its lower tiles
-  constexpr bool B_SYM = MODE == Mode::Poly || MODE == Mode::Mul;  // B likewise
+  // one kernel for all modes: consecutive launches find its code in the caches
+  const Mode mode = g.mode;
+  const bool a_sym = mode != Mode::Gram;                       // A is a symmetric operand
+  const bool b_sym = mode == Mode::Poly || mode == Mode::Mul;  // B likewise
+  const bool b_rows = mode == Mode::Gram;                      // B has K along its rows
   constexpr int BN = PAIR ? 256 : 128;   // tile rows and columns
   constexpr int NC = BN / 2;             // columns of an epilogue warp
   constexpr int CTAS = PAIR ? 2 : 1;
@@ -314,6 +340,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tmem_relinquish();
     }
   }
+  if (warp == 0 && lane == 0 && (int)(blockIdx.x / CTAS) < g.tiles) {
+    const Item& it = g.item[tile_at<BN, CAP>(g, blockIdx.x / CTAS).item];
+    if (!b_rows) {
+      ptx::prefetch_tmap(&it.at);
+      ptx::prefetch_tmap(&it.bt);
+    }
+    ptx::prefetch_tmap(&it.a);
+    if (b_rows || b_sym) ptx::prefetch_tmap(&it.b);
+  }
   ptx::tc_fence_before();
   __syncthreads();
   if (PAIR) ptx::cluster_sync();  // peer barriers initialised, tensor memory allocated
@@ -331,33 +366,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     int unit = 0;
     bool ok = true;
     for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
-      const Tile tile = tile_at<SYM, BN, CAP>(g, t);
+      const Tile tile = tile_at<BN, CAP>(g, t);
       const Item& it = g.item[tile.item];
       // copies: parameters indexed at run time would be fetched at every use
       const int m = it.m, n = it.n, ld = it.ld;
-      const int num_k = (it.k + kBK - 1) / kBK;
+      const int num_k = k_blocks(it, tile);
       const int row0 = tile.m0 + rank * 128 + q * 32, col0 = tile.n0 + cbase;
       const bool live = row0 < m && col0 < n;
       const long long plane = it.plane;
       const long long at = (long long)row0 * ld + col0;
-      const __half* src = MODE == Mode::Poly ? it.g + at : nullptr;
-      if (MODE == Mode::Poly && row0 + lane < m) {
+      const int rows = m - row0;
+      const __half* src = it.g + at;  // Poly
+      float* w = it.w;                // Update
+      const bool tr = it.w_transposed;
+      const long long pitch = tr ? m : n;
+      const float decay = it.decay;
+      // what the epilogue reads, a line per lane, into L2 meanwhile
+      if (mode == Mode::Poly && live) {
+        if (lane < rows)
 #pragma unroll
-        for (int c = 0; c < NC; c += 64) {
-          if (col0 + c < n) {
-            prefetch_l2(src + (long long)lane * ld + c);
-            prefetch_l2(src + plane + (long long)lane * ld + c);
-          }
-        }
+          for (int c = 0; c < NC; c += 64)
+            if (col0 + c < n) {
+              prefetch_l2(src + (long long)lane * ld + c);
+              prefetch_l2(src + plane + (long long)lane * ld + c);
+            }
+      } else if (mode == Mode::Update && live) {
+        w += tr ? col0 * pitch + row0 : row0 * pitch + (long long)col0;
+#pragma unroll
+        for (int c = 0; c < NC; c += 32)
+          if (decay != 0.0f && (tr ? col0 + c + lane < n : lane < rows && col0 + c < n))
+            prefetch_l2(w + (tr ? (c + lane) * pitch : lane * pitch + c));
       }
       float v[NC];
-      Block next;  // the plane of g to be added next; the first before the last segment
+      Block next;  // of g; the first one before the last segment
 #pragma unroll
       for (int i = 0; i < NC; ++i) v[i] = 0.f;
       for (int k0 = 0; k0 < num_k; k0 += kSeg, ++unit) {
         const int acc = unit & 1;
-        if (MODE == Mode::Poly && live && k0 + kSeg >= num_k)
-          load_block(next, lane, src + plane, ld, m - row0);
+        if (mode == Mode::Poly && live && k0 + kSeg >= num_k)
+          load_block(next, lane, src + plane, ld, rows);
         // warp-uniform: every lane takes the same exit
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (unit >> 1) & 1, status, 0x605,
                                                     abort_flag))) {
@@ -385,33 +432,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (!live) continue;
-      if (MODE == Mode::Update) {
-        update_block<NC>(v, stg, lane, it.w, it.w_transposed, it.decay, it.gain, m, n, row0, col0);
-        continue;
-      }
-      const float scale = it.scale;
+      const float scale = mode == Mode::Update ? it.gain : it.scale;
       __half* out = it.out + at;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) v[i] *= scale;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < NC; c += 64) {
         if (col0 + c >= n) break;
-        if (MODE == Mode::Poly) {  // small terms first
-          constexpr float f = kB * (kMScale / kXScale);
-          put_block(next, stg, lane);
-          load_block(next, lane, src + c, ld, m - row0);
-          add_block<NC>(v, c, f, stg, lane);
-          put_block(next, stg, lane);
-          if (c + 64 < NC && col0 + c + 64 < n)
-            load_block(next, lane, src + plane + c + 64, ld, m - row0);
-          add_block<NC>(v, c, f, stg, lane);
-          const int diagonal = row0 + lane - col0 - c;
+        if (mode == Mode::Update) {
+          float* y = w + (tr ? c * pitch : (long long)c);
+          update_block(v, stg, lane, y, pitch, tr, decay, scale, rows, n - col0 - c);
+          if (col0 + c + 32 < n)
+            update_block(v + 32, stg, lane, y + (tr ? 32 * pitch : 32ll), pitch, tr, decay, scale,
+                         rows, n - col0 - c - 32);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i == diagonal) v[c + i] += kA * kMScale;
+          for (int i = 0; i < 64; ++i) v[i] *= scale;
+          if (mode == Mode::Poly) {  // small terms first
+            constexpr float f = kB * (kMScale / kXScale);
+            put_block(next, stg, lane);
+            load_block(next, lane, src + c, ld, rows);
+            add_block(v, f, stg, lane);
+            put_block(next, stg, lane);
+            if (c + 64 < NC && col0 + c + 64 < n)
+              load_block(next, lane, src + plane + c + 64, ld, rows);
+            add_block(v, f, stg, lane);
+            const int diagonal = row0 - col0 - c;  // of the warp's first row
+            if (diagonal > -32 && diagonal < 64) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) v[i] += i == diagonal + lane ? kA * kMScale : 0.f;
+            }
+          }
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+          store_plane(hi, stg, lane, out + c, ld, rows);
+          store_plane(lo, stg, lane, out + plane + c, ld, rows);
         }
-        store_block<0, NC>(v, c, stg, lane, out + c, ld, m - row0);
-        store_block<1, NC>(v, c, stg, lane, out + plane + c, ld, m - row0);
+#pragma unroll
+        for (int i = 0; i < NC - 64; ++i) v[i] = v[i + 64];
       }
     }
   } else {
@@ -423,10 +480,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         long long issued = 0;
         for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
-          const Tile tile = tile_at<SYM, BN, CAP>(g, t);
+          const Tile tile = tile_at<BN, CAP>(g, t);
           const Item& it = g.item[tile.item];
-          const int num_k = (it.k + kBK - 1) / kBK;
+          const int num_k = k_blocks(it, tile);
           const int am = tile.m0 + rank * 128, bn = tile.n0 + rank * 128;
+          const int a_upper = (tile.m0 / kBlock + 1) * kBlock;
+          const int b_upper = (tile.n0 / kBlock + 1) * kBlock;
           for (int kb = 0; kb < num_k; ++kb) {
             if (!ptx::mbar_wait(&empty[stage], phase ^ 1, status, 0x601, abort_flag)) {
               ok = false;
@@ -436,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t* sa = ring + stage * kStage;
             uint8_t* sb = sa + kOperand;
             const int k = kb * kBK;
-            const bool at = A_SYM && k >= tile.m0 + BN, bt = B_SYM ? k >= tile.n0 + BN : !SYM;
+            const bool at = a_sym && k >= a_upper, bt = b_sym ? k >= b_upper : !b_rows;
             if (PAIR) {
               const uint32_t bar = ptx::mapa(ptx::smem_u32(&full[stage]), 0);
               if (at) ptx::tma_load_4d_pair(sa, &it.at, bar, 0, k, am / 64, 0);
@@ -469,8 +528,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int unit = 0;  // segments so far
         bool ok = true;
         for (int t = cluster_id; t < g.tiles && ok; t += n_clusters) {
-          const Tile tile = tile_at<SYM, BN, CAP>(g, t);
-          const int num_k = (g.item[tile.item].k + kBK - 1) / kBK;
+          const Tile tile = tile_at<BN, CAP>(g, t);
+          const int num_k = k_blocks(g.item[tile.item], tile);
+          // K from which a symmetric operand's blocks lie above the diagonal
+          const int a_upper = (tile.m0 / kBlock + 1) * kBlock;
+          const int b_upper = (tile.n0 / kBlock + 1) * kBlock;
           for (int k0 = 0; k0 < num_k && ok; k0 += kSeg, ++unit) {
             const int acc = unit & 1;
             if (!ptx::mbar_wait<PAIR>(&tempty[acc], ((unit >> 1) & 1) ^ 1, status, 0x602,
@@ -488,8 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               ptx::tc_fence_after();
               const uint32_t sa = ptx::smem_u32(ring + stage * kStage), sb = sa + kOperand;
-              const bool at = A_SYM && kb * kBK >= tile.m0 + BN;
-              const bool bt = B_SYM ? kb * kBK >= tile.n0 + BN : !SYM;
+              const bool at = a_sym && kb * kBK >= a_upper;
+              const bool bt = b_sym ? kb * kBK >= b_upper : !b_rows;
               const uint32_t idesc =
                   ptx::make_idesc_f16(CTAS * 128, BN, false, false) | (at << 15) | (bt << 16);
               // K-major: 16 elements = 32 bytes along the swizzled row;

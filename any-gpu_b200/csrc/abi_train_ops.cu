@@ -35,7 +35,7 @@ agpu_status check_len(const agpu_buffer* b, uint64_t want, const char* fn, const
 agpu_status check_embedding(uint64_t tokens, uint32_t vocab, uint32_t dim, const char* fn) {
   if (tokens && vocab == 0) return fail(AGPU_ERR_INVALID, "%s: vocab is 0", fn);
   if (tokens > 0x7fffffffull) return fail(AGPU_ERR_UNSUPPORTED, "%s: too many tokens", fn);
-  if (vocab > 0x7ffff000u || dim > 0x3fffffffu)
+  if (vocab > 0x3fffffffu || dim > 0x3fffffffu)
     return fail(AGPU_ERR_UNSUPPORTED, "%s: table too large", fn);
   return AGPU_OK;
 }

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "agpu_internal.cuh"
+#include "ptx.cuh"
 
 namespace agpu {
 
@@ -22,8 +23,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kIndexWarps = 32;      // warps of an index CTA
 constexpr int kMaxRowsPerCta = 1024; // table rows of an index CTA (one thread scans one)
-constexpr int kChunk = 32;           // sorted positions summed by one CTA
+constexpr int kMinOwners = 128;      // index CTAs, a power of two
+constexpr int kQueue = 64;           // tokens a warp of the index holds back
+constexpr int kJoinGroups = 4;       // groups of a join CTA, each a part of a row's parts
+constexpr int kMaxChunk = 64;        // sorted positions summed by one CTA, at most
 constexpr int kInFlight = 8;         // gradient rows a thread has in flight
+constexpr int kIdsAhead = 8;         // ids a thread of the index has in flight
+constexpr int kFewTokens = 128;      // tokens of the one-launch gradient, at most
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -70,34 +76,114 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // -------------------------------------------------------------- gradient --
-// Stable counting sort of the token positions by id.  Each CTA owns the
-// table rows [lo, lo + rows) and reads all ids itself, twice: it counts its
-// own rows' tokens per warp (a warp owns a contiguous range of positions, so
-// warp order is position order) and the tokens of lower rows, which is where
+// Few tokens: one launch, no scratch.  Each CTA owns `rows` table rows and 256
+// columns, orders the tokens of its rows by (row, position) in shared memory,
+// and writes every element: its sum, or zero.  Bound by launch latency or, for
+// a large table, by the zeros; 37 tokens into 1001 x 99: 6 us, sorting 17.
+template <typename V>
+__global__ void __launch_bounds__(kThreads)
+    embedding_few_kernel(const V* __restrict__ grad, const int* __restrict__ ids,
+                         V* __restrict__ d_table, int tokens, int vocab, int dv, int rows,
+                         int slices, bool accumulate, float scale, unsigned int* status) {
+  __shared__ int id[kFewTokens], list[kFewTokens], first[kThreads + 1];
+  const int tid = threadIdx.x;
+  const int lo = blockIdx.x / slices * rows, n = min(rows, vocab - lo);
+  const int col = blockIdx.x % slices * kThreads + tid;
+  if (tid < tokens) id[tid] = __ldg(ids + tid);
+  __syncthreads();
+  if (tid < tokens) {
+    const int mine = id[tid];
+    if (blockIdx.x == 0 && (mine < -1 || mine >= vocab))
+      atomicCAS(status, 0u, AGPU_BAD_TOKEN_CODE);
+    if (mine >= lo && mine < lo + n) {
+      int rank = 0;
+      for (int u = 0; u < tokens; ++u)
+        rank += id[u] >= lo && (id[u] < mine || (id[u] == mine && u < tid));
+      list[rank] = tid;
+    }
+  }
+  for (int r = tid; r <= n; r += kThreads) {  // tokens of rows before row r, r = 0..n
+    int before = 0;
+    for (int u = 0; u < tokens; ++u) before += id[u] >= lo && id[u] < lo + r;
+    first[r] = before;
+  }
+  __syncthreads();
+  if (col >= dv) return;
+  V* dst = d_table + (long long)lo * dv + col;
+  for (int r = 0; r < n; ++r, dst += dv) {
+    const int p0 = first[r], p1 = first[r + 1];
+    if (p0 == p1) {
+      if (!accumulate) __stcs(dst, zero(V()));
+      continue;
+    }
+    V acc = zero(V());
+    for (int p = p0; p < p1; p += kInFlight) {
+      V g[kInFlight];
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (p + u < p1) g[u] = __ldcs(grad + (long long)list[p + u] * dv + col);
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (p + u < p1) acc = plus(acc, g[u]);
+    }
+    acc = times(acc, scale);
+    if (accumulate) acc = plus(*dst, acc);
+    __stcs(dst, acc);
+  }
+}
+
+// Stable counting sort of the token positions by row.  Row v belongs to CTA
+// v % owners (owners a power of two) as its row v / owners: neighbouring ids,
+// which are the frequent ones in a text's vocabulary, go to different CTAs (with
+// contiguous ranges one CTA had 57% of 65536 such tokens, and took 83 us).  The
+// sorted order is by (v % owners, v / owners, position); only that equal ids
+// are together matters.  Each CTA reads all ids itself, twice: it counts its own
+// rows' tokens per warp (a warp has a contiguous range of positions, so warp
+// order is position order) and the tokens of earlier CTAs' rows, which is where
 // its output starts; then it places its tokens.  No CTA waits for another.
 //   order[p] = token position, sorted[p] = its id, for p in sorted order
-//   starts[v] = first p of row v, starts[vocab] = number of tokens with a row
+//   starts[slot] = first p of the slot of a row (slot_of_row), and behind the
+//   last slot the number of tokens with a row
+struct Owners {
+  int shift, rows;  // owners = 1 << shift, rows of each
+};
+
+__device__ __forceinline__ int slot_of_row(Owners o, int row) {
+  return (row & ((1 << o.shift) - 1)) * o.rows + (row >> o.shift);
+}
+
 __global__ void __launch_bounds__(kIndexWarps * 32)
-    embedding_index_kernel(const int* __restrict__ ids, int tokens, int vocab, int rows,
+    embedding_index_kernel(const int* __restrict__ ids, int tokens, int vocab, Owners own,
                            int* __restrict__ order, int* __restrict__ sorted,
                            int* __restrict__ starts, unsigned int* status) {
   extern __shared__ int count[];  // [kIndexWarps][rows]
   __shared__ int red[kIndexWarps];
+  __shared__ int2 queue[kIndexWarps][kQueue];  // (position, id) of tokens to be placed
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int lo = blockIdx.x * rows, hi = min(lo + rows, vocab);
+  const int rows = own.rows, mask = (1 << own.shift) - 1, me = blockIdx.x;
+  ptx::griddep_launch_dependents();
   for (int i = tid; i < kIndexWarps * rows; i += blockDim.x) count[i] = 0;
   __syncthreads();
+  ptx::griddep_wait();
 
   const int per = ((tokens + kIndexWarps - 1) / kIndexWarps + 31) / 32 * 32;
   const long long p0 = (long long)warp * per;
   const int begin = (int)min((long long)tokens, p0), end = (int)min((long long)tokens, p0 + per);
   int* mine = count + warp * rows;
   int below = 0;
-  for (int i = begin + lane; i < end; i += 32) {
-    const int id = __ldg(ids + i);
-    if (id >= lo && id < hi) atomicAdd(mine + (id - lo), 1);
-    below += id >= 0 && id < lo;
-    if (blockIdx.x == 0 && (id < -1 || id >= vocab)) atomicCAS(status, 0u, AGPU_BAD_TOKEN_CODE);
+  for (int i0 = begin + lane; i0 < end; i0 += 32 * kIdsAhead) {
+    int id[kIdsAhead];
+#pragma unroll
+    for (int u = 0; u < kIdsAhead; ++u)
+      id[u] = i0 + 32 * u < end ? __ldg(ids + i0 + 32 * u) : -1;
+#pragma unroll
+    for (int u = 0; u < kIdsAhead; ++u) {
+      const bool live = (unsigned)id[u] < (unsigned)vocab;
+      const int owner = id[u] & mask;
+      if (live && owner == me) atomicAdd(mine + (id[u] >> own.shift), 1);
+      below += live && owner < me;
+      if (me == 0 && !live && id[u] != -1) atomicCAS(status, 0u, AGPU_BAD_TOKEN_CODE);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
@@ -122,8 +208,8 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
   for (int w = 0; w < warp; ++w) scan += red[w];
   int first = base + scan - total;
   if (tid < rows) {
-    if (lo + tid < vocab) starts[lo + tid] = first;
-    if (lo + tid == vocab - 1) starts[vocab] = first + total;
+    starts[me * rows + tid] = first;
+    if (me == mask && tid == rows - 1) starts[(mask + 1) * rows] = first + total;
     for (int w = 0; w < kIndexWarps; ++w) {  // counts become output offsets
       const int n = count[w * rows + tid];
       count[w * rows + tid] = first;
@@ -132,23 +218,50 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
   }
   __syncthreads();
 
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const int id = i < end ? __ldg(ids + i) : -1;
-    const bool in = id >= lo && id < hi;
-    if (__ballot_sync(0xffffffffu, in) == 0) continue;
-    // lanes with the same row keep their order; other lanes match only themselves
-    const unsigned same = __match_any_sync(0xffffffffu, in ? id : -1 - lane);
+  // A warp's tokens gather in its queue, in order, and are placed 32 at a time:
+  // ranking equal ids among 32 lanes costs the same for one token as for 32.
+  int held = 0;
+  auto place = [&](int n) {
+    const int2 t = lane < n ? queue[warp][lane] : make_int2(0, -1 - lane);
+    const unsigned same = __match_any_sync(0xffffffffu, t.y);
     const int rank = __popc(same & ((1u << lane) - 1));
-    const int at = in ? mine[id - lo] : 0;
+    const int at = lane < n ? mine[t.y >> own.shift] : 0;
     __syncwarp();
-    if (in) {
-      order[at + rank] = i;
-      sorted[at + rank] = id;
-      if (rank == 0) mine[id - lo] = at + __popc(same);
+    if (lane < n) {
+      order[at + rank] = t.x;
+      sorted[at + rank] = t.y;
+      if (rank == 0) mine[t.y >> own.shift] = at + __popc(same);
     }
     __syncwarp();
+  };
+  for (int i0 = begin; i0 < end; i0 += 32 * kIdsAhead) {
+    int id[kIdsAhead];
+#pragma unroll
+    for (int u = 0; u < kIdsAhead; ++u) {
+      const int i = i0 + 32 * u + lane;
+      id[u] = i < end ? __ldg(ids + i) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kIdsAhead; ++u) {
+      const bool in = (unsigned)id[u] < (unsigned)vocab && (id[u] & mask) == me;
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      if (who == 0) continue;
+      if (in)
+        queue[warp][held + __popc(who & ((1u << lane) - 1))] =
+            make_int2(i0 + 32 * u + lane, id[u]);
+      __syncwarp();
+      held += __popc(who);
+      if (held >= 32) {
+        place(32);
+        held -= 32;
+        const int2 rest = lane < held ? queue[warp][32 + lane] : make_int2(0, 0);
+        __syncwarp();
+        if (lane < held) queue[warp][lane] = rest;
+        __syncwarp();
+      }
+    }
   }
+  if (held) place(held);
 }
 
 // CTA b < sum_blocks: chunk b / slices of the sorted positions, columns of
@@ -158,31 +271,34 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
 //   partial[2 * chunk + 1]  the row that begins here and goes on
 // for embedding_join_kernel.  The other CTAs write zeros to the rows without
 // tokens (none of them when accumulating).
-template <typename V>
-__global__ void __launch_bounds__(kThreads)
-    embedding_sum_kernel(const V* __restrict__ grad, const int* __restrict__ order,
-                         const int* __restrict__ sorted, const int* __restrict__ starts,
-                         V* __restrict__ d_table, V* __restrict__ partial, int vocab, int dv,
-                         int slices, long long sum_blocks, int zero_rows, bool accumulate,
-                         float scale) {
+template <typename V, bool ACCUMULATE>
+__global__ void __launch_bounds__(kThreads, 4)
+    embedding_sum_kernel(const V* grad, const int* order, const int* sorted, const int* starts,
+                         V* d_table, V* partial, int vocab,
+                         Owners own, int dv, int slices, int chunk_len, long long sum_blocks,
+                         int zero_rows, float scale) {
+  constexpr int U = ACCUMULATE ? kInFlight / 2 : kInFlight;
   const int tid = threadIdx.x;
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   if ((long long)blockIdx.x >= sum_blocks) {
     const long long v0 = (blockIdx.x - sum_blocks) * zero_rows;
     const int n = (int)min((long long)zero_rows, vocab - v0);
     for (int r = 0; r < n; ++r) {
-      if (__ldg(starts + v0 + r) != __ldg(starts + v0 + r + 1)) continue;
+      const int slot = slot_of_row(own, (int)v0 + r);
+      if (starts[slot] != starts[slot + 1]) continue;
       V* row = d_table + (v0 + r) * dv;
       for (int c = tid; c < dv; c += kThreads) __stcs(row + c, zero(V()));
     }
     return;
   }
-  __shared__ int tok[kChunk], row[kChunk + 2];  // row[0] = the position before the chunk
+  __shared__ int tok[kMaxChunk], row[kMaxChunk + 2];  // row[0] = the position before the chunk
   const long long chunk = blockIdx.x / slices;
   const int col = (int)(blockIdx.x % slices) * kThreads + tid;
-  const int n = __ldg(starts + vocab);
-  const long long p0 = chunk * kChunk;
+  const int n = starts[own.rows << own.shift];
+  const long long p0 = chunk * chunk_len;
   if (p0 >= n) return;
-  const int len = (int)min((long long)kChunk, n - p0);
+  const int len = (int)min((long long)chunk_len, n - p0);
   if (tid < len) tok[tid] = order[p0 + tid];
   if (tid < len + 2) {
     const long long p = p0 - 1 + tid;
@@ -193,26 +309,26 @@ __global__ void __launch_bounds__(kThreads)
 
   bool head = row[0] == row[1];  // the first row began in an earlier chunk
   V acc = zero(V());
-  for (int i0 = 0; i0 < len; i0 += kInFlight) {
-    V g[kInFlight], d[kInFlight];
+  for (int i0 = 0; i0 < len; i0 += U) {
+    V g[U], d[U];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int i = i0 + u;
       if (i < len) {
         g[u] = __ldcs(grad + (long long)tok[i] * dv + col);
-        if (accumulate && row[i + 1] != row[i + 2])
+        if (ACCUMULATE && row[i + 1] != row[i + 2])
           d[u] = d_table[(long long)row[i + 1] * dv + col];
       }
     }
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int i = i0 + u;
       if (i < len) {
         acc = plus(acc, g[u]);
         const bool ends = row[i + 1] != row[i + 2];
         if (ends && !head) {
           V y = times(acc, scale);
-          if (accumulate) y = plus(d[u], y);
+          if (ACCUMULATE) y = plus(d[u], y);
           __stcs(d_table + (long long)row[i + 1] * dv + col, y);
         } else if (ends || i == len - 1) {
           partial[(2 * chunk + (head ? 0 : 1)) * dv + col] = acc;
@@ -227,35 +343,68 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The rows that cross chunks: the CTAs of the chunk a row begins in add its
-// parts in chunk order.
+// parts.  A frequent token's row has hundreds of them, so each of a CTA's
+// groups adds a contiguous quarter in chunk order, and the quarters follow.
 template <typename V>
 __global__ void __launch_bounds__(kThreads)
-    embedding_join_kernel(const int* __restrict__ sorted, const int* __restrict__ starts,
-                          const V* __restrict__ partial, V* __restrict__ d_table, int vocab,
-                          int dv, int slices, bool accumulate, float scale) {
+    embedding_join_kernel(const int* sorted, const int* starts, const V* partial, V* d_table,
+                          Owners own,
+                          int dv, int slices, int chunk_len, bool accumulate, float scale) {
+  constexpr int kCols = kThreads / kJoinGroups;
+  __shared__ V sums[kJoinGroups][kCols];
   const long long chunk = blockIdx.x / slices;
-  const int col = (int)(blockIdx.x % slices) * kThreads + threadIdx.x;
-  const int n = __ldg(starts + vocab);
-  const long long p1 = (chunk + 1) * kChunk;
-  if (p1 >= n || col >= dv) return;
-  const int row = __ldg(sorted + p1);
-  const int first = __ldg(starts + row);
-  if (first < chunk * kChunk || first >= p1) return;  // begins in another chunk
-  const long long last = (__ldg(starts + row + 1) - 1) / kChunk;
-  V acc = partial[(2 * chunk + 1) * dv + col];
-  for (long long k = chunk + 1; k <= last; k += kInFlight) {
-    V part[kInFlight];
+  const int group = threadIdx.x / kCols, lane = threadIdx.x % kCols;
+  const int col = (int)(blockIdx.x % slices) * kCols + lane;
+  ptx::griddep_wait();
+  const int n = starts[own.rows << own.shift];
+  const long long p1 = (chunk + 1) * chunk_len;
+  if (p1 >= n) return;
+  const int row = sorted[p1];
+  const int slot = slot_of_row(own, row), first = starts[slot];
+  if (first < chunk * chunk_len || first >= p1) return;  // begins in another chunk
+  // part 0 is the chunk's own, part k the head of chunk `chunk + k`
+  const int parts = (int)((starts[slot + 1] - 1) / chunk_len - chunk) + 1;
+  const int per = (parts + kJoinGroups - 1) / kJoinGroups;
+  V acc = zero(V());
+  if (col < dv) {
+    const int end = min(parts, (group + 1) * per);
+    for (int k = group * per; k < end; k += kInFlight) {
+      V part[kInFlight];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u)
-      if (k + u <= last) part[u] = partial[2 * (k + u) * dv + col];
+      for (int u = 0; u < kInFlight; ++u)
+        if (k + u < end) part[u] = partial[(2 * (chunk + k + u) + (k + u == 0)) * dv + col];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u)
-      if (k + u <= last) acc = plus(acc, part[u]);
+      for (int u = 0; u < kInFlight; ++u)
+        if (k + u < end) acc = plus(acc, part[u]);
+    }
   }
+  sums[group][lane] = acc;
+  __syncthreads();
+  if (group != 0 || col >= dv) return;
+#pragma unroll
+  for (int g = 1; g < kJoinGroups; ++g) acc = plus(acc, sums[g][lane]);
   V y = times(acc, scale);
   V* dst = d_table + (long long)row * dv + col;
   if (accumulate) y = plus(*dst, y);
   *dst = y;
+}
+
+// Launches a kernel that may start while the one before it in the stream ends
+// (it waits for it with griddepcontrol before it touches memory).
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), uint64_t grid, int block, int smem,
+                         cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
 template <typename V>
@@ -281,42 +430,62 @@ template <typename V>
 agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids, float* d_table,
                      int tokens, int vocab, uint32_t dv, float scale, bool accumulate,
                      cudaStream_t s) {
-  const int rows = (int)std::min<uint64_t>(
-      kMaxRowsPerCta, std::max<uint64_t>(32, ceil_div(vocab, dev->sm_count)));
-  const uint64_t chunks = ceil_div(tokens, kChunk), slices = ceil_div(dv, kThreads);
+  if (tokens <= kFewTokens) {
+    const uint64_t slices = ceil_div(dv, kThreads);
+    const uint64_t per = std::min<uint64_t>(
+        kThreads, std::max<uint64_t>(1, vocab * slices / (8ull * dev->sm_count)));
+    const uint64_t blocks = ceil_div(vocab, per) * slices;
+    if (blocks > 0x7fffffffull)
+      return fail(AGPU_ERR_UNSUPPORTED, "embedding_backward: too large");
+    embedding_few_kernel<V><<<(unsigned)blocks, kThreads, 0, s>>>(
+        reinterpret_cast<const V*>(grad_out), ids, reinterpret_cast<V*>(d_table), tokens, vocab,
+        (int)dv, (int)per, (int)slices, accumulate, scale, dev->d_status);
+    return after_launch(dev, "embedding_few_kernel");
+  }
+  Owners own = {0, 0};
+  while ((1 << own.shift) < kMinOwners ||
+         ceil_div(vocab, 1ull << own.shift) > (uint64_t)kMaxRowsPerCta)
+    ++own.shift;
+  own.rows = (int)ceil_div(vocab, 1ull << own.shift);
+  const uint64_t slots = (uint64_t)own.rows << own.shift;
+  const uint64_t slices = ceil_div(dv, kThreads);
+  // long chunks leave fewer parts to join, if there are enough of them
+  const int chunk_len =
+      ceil_div(tokens, kMaxChunk) * slices >= 4ull * dev->sm_count ? kMaxChunk : kMaxChunk / 2;
+  const uint64_t chunks = ceil_div(tokens, chunk_len);
   const uint64_t sum_blocks = chunks * slices;
+  const uint64_t join_slices = ceil_div(dv, kThreads / kJoinGroups);
   const int zero_rows = std::max<int>(1, 4096 / (int)dv);
   const uint64_t zero_blocks = accumulate ? 0 : ceil_div(vocab, zero_rows);
-  if (sum_blocks + zero_blocks > 0x7fffffffull)
+  if (sum_blocks + zero_blocks > 0x7fffffffull || chunks * join_slices > 0x7fffffffull)
     return fail(AGPU_ERR_UNSUPPORTED, "embedding_backward: too large");
-  const size_t ints = (2ull * tokens + vocab + 1 + 3) / 4 * 4;
+  const size_t ints = (2ull * tokens + slots + 1 + 3) / 4 * 4;
   void* scratch = nullptr;
   AGPU_TRY(pool_alloc(dev, ints * 4 + 2 * chunks * dv * sizeof(V), &scratch, s));
   int* order = static_cast<int*>(scratch);
   int *sorted = order + tokens, *starts = sorted + tokens;
   V* partial = reinterpret_cast<V*>(order + ints);
-  const int smem = kIndexWarps * rows * (int)sizeof(int);
-  cudaError_t e =
-      set_smem_once<embedding_index_kernel>(dev, kIndexWarps * kMaxRowsPerCta * sizeof(int));
-  agpu_status st = e == cudaSuccess ? AGPU_OK : cuda_status(e, "embedding_backward");
-  if (st == AGPU_OK) {
-    embedding_index_kernel<<<(unsigned)ceil_div(vocab, rows), kIndexWarps * 32, smem, s>>>(
-        ids, tokens, vocab, rows, order, sorted, starts, dev->d_status);
-    st = after_launch(dev, "embedding_index_kernel");
-  }
   const V* g = reinterpret_cast<const V*>(grad_out);
   V* d = reinterpret_cast<V*>(d_table);
-  if (st == AGPU_OK) {
-    embedding_sum_kernel<V><<<(unsigned)(sum_blocks + zero_blocks), kThreads, 0, s>>>(
-        g, order, sorted, starts, d, partial, vocab, (int)dv, (int)slices, (long long)sum_blocks,
-        zero_rows, accumulate, scale);
-    st = after_launch(dev, "embedding_sum_kernel");
-  }
-  if (st == AGPU_OK && chunks > 1) {
-    embedding_join_kernel<V><<<(unsigned)sum_blocks, kThreads, 0, s>>>(
-        sorted, starts, partial, d, vocab, (int)dv, (int)slices, accumulate, scale);
-    st = after_launch(dev, "embedding_join_kernel");
-  }
+  auto run = [&]() -> agpu_status {
+    AGPU_CUDA(set_smem_once<embedding_index_kernel>(dev,
+                                                    kIndexWarps * kMaxRowsPerCta * sizeof(int)));
+    AGPU_CUDA(launch_after(embedding_index_kernel, 1ull << own.shift, kIndexWarps * 32,
+                           kIndexWarps * own.rows * (int)sizeof(int), s, ids, tokens, vocab, own,
+                           order, sorted, starts, dev->d_status));
+    AGPU_TRY(after_launch(dev, "embedding_index_kernel"));
+    auto sum = accumulate ? embedding_sum_kernel<V, true> : embedding_sum_kernel<V, false>;
+    AGPU_CUDA(launch_after(sum, sum_blocks + zero_blocks, kThreads, 0, s, g, order, sorted, starts,
+                           d, partial, vocab, own, (int)dv, (int)slices, chunk_len,
+                           (long long)sum_blocks, zero_rows, scale));
+    AGPU_TRY(after_launch(dev, "embedding_sum_kernel"));
+    if (chunks == 1) return AGPU_OK;
+    AGPU_CUDA(launch_after(embedding_join_kernel<V>, chunks * join_slices, kThreads, 0, s, sorted,
+                           starts, partial, d, own, (int)dv, (int)join_slices, chunk_len,
+                           accumulate, scale));
+    return after_launch(dev, "embedding_join_kernel");
+  };
+  const agpu_status st = run();
   pool_free(dev, scratch, s);
   return st;
 }

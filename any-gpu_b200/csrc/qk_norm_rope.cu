@@ -34,8 +34,7 @@ struct Args {
   const float* w[2];  // weights or null (ones)
   Strides in[2], out[2];
   int heads[2];
-  int units[2];   // vector kernels: warp units per token
-  int per_unit;   // heads per warp unit
+  int batches[2];  // vector kernels: warp batches per token
   const int* positions;
   long long tokens;
   int seq, dim, rot;
@@ -127,147 +126,198 @@ __device__ __forceinline__ void turns_of(const double (&f)[4], const Slot& sl, i
   }
 }
 
-// A warp unit is one token's next `per_unit` query or key heads; a warp walks
-// units with the grid's stride and keeps its slot's frequencies.
-__global__ void __launch_bounds__(kThreads) qk_forward_vec_kernel(const __grid_constant__ Args a,
-                                                                  int lanes) {
-  constexpr int J = 4;
-  const int lane = threadIdx.x % 32, group = lane / lanes, groups = 32 / lanes;
-  const Slot sl = slot_of(lane % lanes, a.dim, a.rot);
-  const float inv_dim = 1.0f / (float)a.dim;
-  double f[4];
-  for (int i = 0; i < 4; ++i) f[i] = sl.turns ? inv_freq_of(sl.a + i, a.rot, a.log2_base) : 0.0;
-  const int per_token = a.units[0] + a.units[1];
-  const long long units = a.tokens * per_token;
-  for (long long u = blockIdx.x * (long long)kWarps + threadIdx.x / 32; u < units;
-       u += (long long)gridDim.x * kWarps) {
-    const long long token = u / per_token;
-    const int part = (int)(u - token * per_token);
-    const int k = part >= a.units[0];
-    const int h0 = (k ? part - a.units[0] : part) * a.per_unit;
-    const int h1 = min(h0 + a.per_unit, a.heads[k]);
-    const long long b = token / a.seq, s = token - b * a.seq;
-    const float* x = a.x[k] + offset(a.in[k], b, s, 0);
-    float* y = a.y[k] + offset(a.out[k], b, s, 0);
-    float4 c, sn;
-    turns_of(f, sl, position_of(a, token), c, sn);
-    float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa;
-    if (a.w[k] && sl.live) {
-      wa = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.a));
-      wb = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.b));
-    }
-    for (int hb = h0; hb < h1; hb += groups * J) {
-      float4 xa[J], xb[J];
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int h = hb + j * groups + group;
-        xa[j] = xb[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h < h1 && sl.live) {
-          xa[j] = ldg4(x + h * a.in[k].head + sl.a);
-          xb[j] = ldg4(x + h * a.in[k].head + sl.b);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int h = hb + j * groups + group;
-        const float ss = group_sum(dot4(xa[j], xa[j]) + dot4(xb[j], xb[j]), lanes);
-        const float r = 1.0f / sqrtf(ss * inv_dim + a.eps);
-        const float4 ya = mul4(mul4(xa[j], r), wa), yb = mul4(mul4(xb[j], r), wb);
-        if (h < h1 && sl.live) {
-          st4(y + h * a.out[k].head + sl.a, fma4(neg4(yb), sn, mul4(ya, c)));
-          st4(y + h * a.out[k].head + sl.b, fma4(ya, sn, mul4(yb, c)));
-        }
-      }
-    }
+// Vector kernels: a batch is the next J * 32 / lanes query or key heads of a
+// token, one head per group of lanes and j < J.  A warp takes a contiguous
+// range of all batches (tokens in order, their queries first), so warps differ
+// by one batch at most and neighbouring batches share their angles.  The
+// operands of the next batch are on their way into shared memory (cp.async, 16
+// bytes a lane, read by the lane that copied them: no barrier) while one is
+// worked on: 8 KB in flight per warp without holding registers.  With the
+// loads in registers the backward kernel needed 152 of them and reached 47% of
+// the DRAM bandwidth.
+constexpr int kPieces = 8;  // float4 per lane and batch
+constexpr int kStages = 3;  // batches in shared memory: one worked on, the others on their way
+constexpr int kCtas = 4;    // CTAs on an SM
+
+struct Batch {
+  long long token, b, s;
+  int part;  // of the token: queries' batches, then keys'
+  int k, h;  // queries or keys; this lane's first head
+};
+
+__device__ __forceinline__ void at_batch(const Args& a, Batch& t, long long i, int per_token) {
+  t.token = i / per_token;
+  t.part = (int)(i - t.token * per_token);
+  t.b = t.token / a.seq;
+  t.s = t.token - t.b * a.seq;
+}
+
+__device__ __forceinline__ void next_batch(const Args& a, Batch& t, int per_token) {
+  if (++t.part < per_token) return;
+  t.part = 0;
+  ++t.token;
+  if (++t.s == a.seq) {
+    t.s = 0;
+    ++t.b;
   }
 }
 
-// The same units; each lane also sums its slot's weight gradients over all
-// units of its warp, and the CTA's warps add theirs in warp order.
-__global__ void __launch_bounds__(kThreads) qk_backward_vec_kernel(const __grid_constant__ Args a,
-                                                                   int lanes) {
-  constexpr int J = 2;
-  __shared__ float4 red[kWarps][32][2];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+__device__ __forceinline__ void copy16(float4* dst, const float* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
+}
+
+// J heads per lane group and batch: 2 operands (x, and g backward) x 2 float4.
+template <bool BACKWARD>
+__global__ void __launch_bounds__(kThreads, kCtas) qk_vec_kernel(const __grid_constant__ Args a,
+                                                             int lanes, int warps) {
+  constexpr int J = BACKWARD ? 2 : 4;
+  extern __shared__ float4 dyn[];  // [kStages][kPieces][kThreads]
+  float4(*buf)[kPieces][kThreads] = reinterpret_cast<float4(*)[kPieces][kThreads]>(dyn);
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int group = lane / lanes, groups = 32 / lanes;
   const Slot sl = slot_of(lane % lanes, a.dim, a.rot);
   const float inv_dim = 1.0f / (float)a.dim;
-  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), one = make_float4(1.f, 1.f, 1.f, 1.f);
+  const int per_token = a.batches[0] + a.batches[1];
+  const long long all = a.tokens * per_token, w = blockIdx.x * (long long)kWarps + warp;
+  long long i = w < warps ? w * all / warps : 0;
+  const long long end = w < warps ? (w + 1) * all / warps : 0;
+
+  // this lane's heads of a batch, and its copies into a stage
+  auto heads_of = [&](Batch& t) {
+    t.k = t.part >= a.batches[0];
+    t.h = (t.k ? t.part - a.batches[0] : t.part) * groups * J + group;
+  };
+  auto fetch = [&](Batch& t, int stage) {
+    heads_of(t);
+    const float* x = a.x[t.k] + offset(a.in[t.k], t.b, t.s, t.h);
+    const float* g = BACKWARD ? a.g[t.k] + offset(a.out[t.k], t.b, t.s, t.h) : nullptr;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (t.h + j * groups < a.heads[t.k] && sl.live) {
+        copy16(&buf[stage][2 * j][tid], x + sl.a);
+        copy16(&buf[stage][2 * j + 1][tid], x + sl.b);
+        if (BACKWARD) {
+          copy16(&buf[stage][2 * J + 2 * j][tid], g + sl.a);
+          copy16(&buf[stage][2 * J + 2 * j + 1][tid], g + sl.b);
+        }
+      }
+      x += groups * a.in[t.k].head;
+      if (BACKWARD) g += groups * a.out[t.k].head;
+    }
+  };
+
+  Batch cur = {}, ahead;
+  if (i < end) at_batch(a, cur, i, per_token);
+  ahead = cur;
+#pragma unroll
+  for (int p = 0; p < kStages - 1; ++p) {
+    if (i + p < end) {
+      fetch(ahead, p);
+      next_batch(a, ahead, per_token);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   double f[4];
-  for (int i = 0; i < 4; ++i) f[i] = sl.turns ? inv_freq_of(sl.a + i, a.rot, a.log2_base) : 0.0;
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    float4 dwa = zero, dwb = zero;
-    const long long units = a.tokens * a.units[k];
-    for (long long u = blockIdx.x * (long long)kWarps + warp; u < units;
-         u += (long long)gridDim.x * kWarps) {
-      const long long token = u / a.units[k];
-      const int h0 = (int)(u - token * a.units[k]) * a.per_unit;
-      const int h1 = min(h0 + a.per_unit, a.heads[k]);
-      const long long b = token / a.seq, s = token - b * a.seq;
-      const float* x = a.x[k] + offset(a.in[k], b, s, 0);
-      const float* g = a.g[k] + offset(a.out[k], b, s, 0);
-      float* y = a.y[k] + offset(a.in[k], b, s, 0);
-      float4 c, sn;
-      turns_of(f, sl, position_of(a, token), c, sn);
-      float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa;
-      if (a.w[k] && sl.live) {
-        wa = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.a));
-        wb = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.b));
-      }
-      for (int hb = h0; hb < h1; hb += groups * J) {
-        float4 xa[J], xb[J], ga[J], gb[J];
+  for (int e = 0; e < 4; ++e) f[e] = sl.turns ? inv_freq_of(sl.a + e, a.rot, a.log2_base) : 0.0;
+  float4 dw[2][2] = {{zero, zero}, {zero, zero}};  // weights' gradients: queries, keys
+  float4 c, sn;           // cos and sin of a token
+  long long turned = -1;  // which
+  // forward: the weights' products with cos and sin, of queries or keys
+  float4 ac, as, bc, bs;
+  int folded = -1;
+  for (int stage = 0; i < end; ++i) {
+    if (i + kStages - 1 < end) {
+      fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);
+      next_batch(a, ahead, per_token);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    heads_of(cur);
+    if (turned != cur.token) {
+      turned = cur.token;
+      turns_of(f, sl, position_of(a, cur.token), c, sn);
+      folded = -1;
+    }
+    const int k = cur.k;
+    float4 wa = one, wb = one;
+    if ((BACKWARD || folded != k) && a.w[k] && sl.live) {
+      wa = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.a));
+      wb = __ldg(reinterpret_cast<const float4*>(a.w[k] + sl.b));
+    }
+    if (!BACKWARD && folded != k) {
+      folded = k;
+      ac = mul4(wa, c);
+      as = mul4(wa, sn);
+      bc = mul4(wb, c);
+      bs = neg4(mul4(wb, sn));
+    }
+    const Strides& to = BACKWARD ? a.in[k] : a.out[k];
+    float* y = a.y[k] + offset(to, cur.b, cur.s, cur.h);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int h = hb + j * groups + group;
-          xa[j] = xb[j] = ga[j] = gb[j] = zero;
-          if (h < h1 && sl.live) {
-            xa[j] = ldg4(x + h * a.in[k].head + sl.a);
-            xb[j] = ldg4(x + h * a.in[k].head + sl.b);
-            ga[j] = ldg4(g + h * a.out[k].head + sl.a);
-            gb[j] = ldg4(g + h * a.out[k].head + sl.b);
-          }
+    for (int j = 0; j < J; ++j, y += groups * to.head) {
+      const bool in = cur.h + j * groups < a.heads[k] && sl.live;
+      const float4 xa = in ? buf[stage][2 * j][tid] : zero;
+      const float4 xb = in ? buf[stage][2 * j + 1][tid] : zero;
+      float ss = dot4(xa, xa) + dot4(xb, xb);
+      if (!BACKWARD) {
+        const float r = rsqrtf(group_sum(ss, lanes) * inv_dim + a.eps);
+        if (in) {
+          st4(y + sl.a, mul4(fma4(xb, bs, mul4(xa, ac)), r));
+          st4(y + sl.b, mul4(fma4(xa, as, mul4(xb, bc)), r));
         }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int h = hb + j * groups + group;
-          const float4 ua = fma4(gb[j], sn, mul4(ga[j], c));        // rotated back
-          const float4 ub = fma4(neg4(ga[j]), sn, mul4(gb[j], c));
-          const float4 ha = mul4(ua, wa), hbv = mul4(ub, wb);
-          float ss = dot4(xa[j], xa[j]) + dot4(xb[j], xb[j]);
-          float hx = dot4(ha, xa[j]) + dot4(hbv, xb[j]);
-          ss = group_sum(ss, lanes);
-          hx = group_sum(hx, lanes);
-          const float r = 1.0f / sqrtf(ss * inv_dim + a.eps);
-          const float4 na = mul4(xa[j], r), nb = mul4(xb[j], r);
-          const float m = -(hx * r) * inv_dim;  // -mean(h x r)
-          const float4 mm = make_float4(m, m, m, m);
-          if (h < h1 && sl.live) {
-            st4(y + h * a.in[k].head + sl.a, mul4(fma4(na, mm, ha), r));
-            st4(y + h * a.in[k].head + sl.b, mul4(fma4(nb, mm, hbv), r));
-            dwa = fma4(ua, na, dwa);
-            dwb = fma4(ub, nb, dwb);
+      } else {
+        const float4 ga = in ? buf[stage][2 * J + 2 * j][tid] : zero;
+        const float4 gb = in ? buf[stage][2 * J + 2 * j + 1][tid] : zero;
+        const float4 ua = fma4(gb, sn, mul4(ga, c));  // rotated back
+        const float4 ub = fma4(neg4(ga), sn, mul4(gb, c));
+        const float4 ha = mul4(ua, wa), hb = mul4(ub, wb);
+        float hx = dot4(ha, xa) + dot4(hb, xb);
+        ss = group_sum(ss, lanes);
+        hx = group_sum(hx, lanes);
+        const float r = rsqrtf(ss * inv_dim + a.eps);
+        const float4 na = mul4(xa, r), nb = mul4(xb, r);
+        const float m = -(hx * r) * inv_dim;  // -mean(h x r)
+        const float4 mm = make_float4(m, m, m, m);
+        if (in) {
+          st4(y + sl.a, mul4(fma4(na, mm, ha), r));
+          st4(y + sl.b, mul4(fma4(nb, mm, hb), r));
+          if (k) {
+            dw[1][0] = fma4(ua, na, dw[1][0]);
+            dw[1][1] = fma4(ub, nb, dw[1][1]);
+          } else {
+            dw[0][0] = fma4(ua, na, dw[0][0]);
+            dw[0][1] = fma4(ub, nb, dw[0][1]);
           }
         }
       }
     }
-    if (!a.partial) continue;
-    __syncthreads();
-    red[warp][lane][0] = dwa;
-    red[warp][lane][1] = dwb;
-    __syncthreads();
-    if (threadIdx.x < lanes && sl.live) {  // lane == slot: sum groups and warps in order
-      dwa = dwb = zero;
-      for (int w = 0; w < kWarps; ++w)
-        for (int gr = 0; gr < groups; ++gr) {
-          const float4 pa = red[w][gr * lanes + lane][0], pb = red[w][gr * lanes + lane][1];
-          dwa = make_float4(dwa.x + pa.x, dwa.y + pa.y, dwa.z + pa.z, dwa.w + pa.w);
-          dwb = make_float4(dwb.x + pb.x, dwb.y + pb.y, dwb.z + pb.z, dwb.w + pb.w);
-        }
-      float* p = a.partial + ((long long)blockIdx.x * 2 + k) * a.dim;
-      *reinterpret_cast<float4*>(p + sl.a) = dwa;
-      *reinterpret_cast<float4*>(p + sl.b) = dwb;
-    }
+    next_batch(a, cur, per_token);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!BACKWARD || !a.partial) return;
+  // the CTA's sums: groups and warps in order
+  float4(*red)[32][4] = reinterpret_cast<float4(*)[32][4]>(dyn);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) red[warp][lane][2 * k + h] = dw[k][h];
+  __syncthreads();
+  if (warp < 2 && lane < lanes && sl.live) {  // warp = queries or keys, lane = slot
+    float4 pa = zero, pb = zero;
+    for (int v = 0; v < kWarps; ++v)
+      for (int gr = 0; gr < groups; ++gr) {
+        pa = fma4(one, red[v][gr * lanes + lane][2 * warp], pa);
+        pb = fma4(one, red[v][gr * lanes + lane][2 * warp + 1], pb);
+      }
+    float* p = a.partial + (blockIdx.x * 2ll + warp) * a.dim;
+    *reinterpret_cast<float4*>(p + sl.a) = pa;
+    *reinterpret_cast<float4*>(p + sl.b) = pb;
   }
 }
 
@@ -353,8 +403,10 @@ __global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const float* __res
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int col = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (col < 2 * dim)
+  if (col < 2 * dim) {
+#pragma unroll 8
     for (int p = warp; p < parts; p += 32) v += partial[(long long)p * 2 * dim + col];
+  }
   red[warp][lane] = v;
   __syncthreads();
   if (warp != 0 || col >= 2 * dim) return;
@@ -411,16 +463,14 @@ int lanes_for(int dim) {
   return lanes;
 }
 
-// Heads per warp unit: as many as leave every SM 32 warps, so that a unit's
-// angles serve several heads.
-void split_units(Args& a, int lanes, int sm_count) {
-  const int groups = 32 / lanes;
-  a.per_unit = groups * 8;
-  for (;;) {
-    for (int k = 0; k < 2; ++k) a.units[k] = (a.heads[k] + a.per_unit - 1) / a.per_unit;
-    if (a.per_unit <= groups || a.tokens * (a.units[0] + a.units[1]) >= 32ll * sm_count) return;
-    a.per_unit /= 2;
-  }
+constexpr int kVecSmem = kStages * kPieces * kThreads * sizeof(float4);
+
+// Batches per token, and the warps that share all of them.
+int split_batches(Args& a, int lanes, int j, int sm_count) {
+  const int heads = 32 / lanes * j;
+  for (int k = 0; k < 2; ++k) a.batches[k] = (a.heads[k] + heads - 1) / heads;
+  return (int)std::min<long long>(a.tokens * (a.batches[0] + a.batches[1]),
+                                  (long long)kCtas * kWarps * sm_count);
 }
 
 }  // namespace
@@ -435,10 +485,9 @@ agpu_status launch_qk_norm_rope(agpu_device* dev, const agpu_qk_norm_rope& d, co
   if (a.tokens == 0 || a.heads[0] + a.heads[1] == 0) return AGPU_OK;
   if (vector_ok(a)) {
     const int lanes = lanes_for(a.dim);
-    split_units(a, lanes, dev->sm_count);
-    const long long want = (a.tokens * (a.units[0] + a.units[1]) + kWarps - 1) / kWarps;
-    const unsigned grid = (unsigned)std::min<long long>(want, 6ll * dev->sm_count);
-    qk_forward_vec_kernel<<<grid, kThreads, 0, s>>>(a, lanes);
+    const int warps = split_batches(a, lanes, 4, dev->sm_count);
+    AGPU_CUDA(set_smem_once<qk_vec_kernel<false>>(dev, kVecSmem));
+    qk_vec_kernel<false><<<(warps + kWarps - 1) / kWarps, kThreads, kVecSmem, s>>>(a, lanes, warps);
   } else {
     const unsigned grid = (unsigned)std::min<long long>(a.tokens, 16ll * dev->sm_count);
     qk_any_kernel<false><<<grid, kThreads, a.rot * sizeof(float), s>>>(a);
@@ -465,20 +514,21 @@ agpu_status launch_qk_norm_rope_backward(agpu_device* dev, const agpu_qk_norm_ro
   const bool vec = vector_ok(a);
   const int lanes = lanes_for(a.dim);
   unsigned grid;
+  int warps = 0;
   if (vec) {
-    split_units(a, lanes, dev->sm_count);
-    const long long most = a.tokens * std::max(a.units[0], a.units[1]);
-    grid = (unsigned)std::min<long long>((most + kWarps - 1) / kWarps, 6ll * dev->sm_count);
+    warps = split_batches(a, lanes, 2, dev->sm_count);
+    grid = (warps + kWarps - 1) / kWarps;
   } else {
     grid = (unsigned)std::min<long long>(a.tokens, 4ll * dev->sm_count);
   }
+  if (vec) AGPU_CUDA(set_smem_once<qk_vec_kernel<true>>(dev, kVecSmem));
   void* scratch = nullptr;
   if (d_q_weight || d_k_weight) {
     AGPU_TRY(pool_alloc(dev, (size_t)grid * 2 * a.dim * sizeof(float), &scratch, s));
     a.partial = static_cast<float*>(scratch);
   }
   if (vec) {
-    qk_backward_vec_kernel<<<grid, kThreads, 0, s>>>(a, lanes);
+    qk_vec_kernel<true><<<grid, kThreads, kVecSmem, s>>>(a, lanes, warps);
   } else {
     const size_t smem = (a.rot + kWarps * 2 * a.dim) * sizeof(float);
     qk_any_kernel<true><<<grid, kThreads, smem, s>>>(a);

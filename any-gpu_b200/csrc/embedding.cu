@@ -264,8 +264,9 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
   if (held) place(held);
 }
 
-// CTA b < sum_blocks: chunk b / slices of the sorted positions, columns of
-// slice b % slices (one V per thread).  Rows that lie inside the chunk are
+// CTA b < sum_blocks: 256 / lanes neighbouring chunks of the sorted positions
+// (one if a row has 256 V or more), columns of slice b % slices, one V per
+// thread.  Rows that lie inside the chunk are
 // written; a row that crosses into or out of it leaves its part in
 //   partial[2 * chunk]      the row that began in an earlier chunk
 //   partial[2 * chunk + 1]  the row that begins here and goes on
@@ -275,37 +276,39 @@ template <typename V, bool ACCUMULATE>
 __global__ void __launch_bounds__(kThreads, 4)
     embedding_sum_kernel(const V* grad, const int* order, const int* sorted, const int* starts,
                          V* d_table, V* partial, int vocab,
-                         Owners own, int dv, int slices, int chunk_len, long long sum_blocks,
-                         int zero_rows, float scale) {
+                         Owners own, int dv, int slices, int lanes, int chunk_len,
+                         long long sum_blocks, int zero_rows, float scale) {
   constexpr int U = ACCUMULATE ? kInFlight / 2 : kInFlight;
+  __shared__ int toks[kThreads / 32][kMaxChunk], rows[kThreads / 32][kMaxChunk + 2];
   const int tid = threadIdx.x;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   if ((long long)blockIdx.x >= sum_blocks) {
     const long long v0 = (blockIdx.x - sum_blocks) * zero_rows;
-    const int n = (int)min((long long)zero_rows, vocab - v0);
-    for (int r = 0; r < n; ++r) {
-      const int slot = slot_of_row(own, (int)v0 + r);
-      if (starts[slot] != starts[slot + 1]) continue;
-      V* row = d_table + (v0 + r) * dv;
-      for (int c = tid; c < dv; c += kThreads) __stcs(row + c, zero(V()));
+    const int n = (int)min((long long)zero_rows, vocab - v0) * dv;
+    V* base = d_table + v0 * dv;
+#pragma unroll 4
+    for (int i = tid; i < n; i += kThreads) {
+      const int slot = slot_of_row(own, (int)v0 + i / dv);
+      if (starts[slot] == starts[slot + 1]) __stcs(base + i, zero(V()));
     }
     return;
   }
-  __shared__ int tok[kMaxChunk], row[kMaxChunk + 2];  // row[0] = the position before the chunk
-  const long long chunk = blockIdx.x / slices;
-  const int col = (int)(blockIdx.x % slices) * kThreads + tid;
+  const int group = tid / lanes, lane = tid % lanes;
+  const long long chunk = blockIdx.x / slices * (long long)(kThreads / lanes) + group;
+  const int col = (int)(blockIdx.x % slices) * kThreads + lane;
   const int n = starts[own.rows << own.shift];
   const long long p0 = chunk * chunk_len;
-  if (p0 >= n) return;
-  const int len = (int)min((long long)chunk_len, n - p0);
-  if (tid < len) tok[tid] = order[p0 + tid];
-  if (tid < len + 2) {
-    const long long p = p0 - 1 + tid;
-    row[tid] = p >= 0 && p < n ? sorted[p] : -1;
-  }
+  const int len = (int)max(0ll, min((long long)chunk_len, n - p0));
+  int *tok = toks[group], *row = rows[group];  // row[0] = the position before the chunk
+  for (int i = lane; i < len; i += lanes) tok[i] = order[p0 + i];
+  if (len > 0)
+    for (int i = lane; i < len + 2; i += lanes) {
+      const long long p = p0 - 1 + i;
+      row[i] = p >= 0 && p < n ? sorted[p] : -1;
+    }
   __syncthreads();
-  if (col >= dv) return;
+  if (col >= dv || len == 0) return;
 
   bool head = row[0] == row[1];  // the first row began in an earlier chunk
   V acc = zero(V());
@@ -453,7 +456,9 @@ agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids
   const int chunk_len =
       ceil_div(tokens, kMaxChunk) * slices >= 4ull * dev->sm_count ? kMaxChunk : kMaxChunk / 2;
   const uint64_t chunks = ceil_div(tokens, chunk_len);
-  const uint64_t sum_blocks = chunks * slices;
+  int lanes = 32;
+  while (lanes < (int)dv && lanes < kThreads) lanes *= 2;
+  const uint64_t sum_blocks = ceil_div(chunks, kThreads / lanes) * slices;
   const uint64_t join_slices = ceil_div(dv, kThreads / kJoinGroups);
   const int zero_rows = std::max<int>(1, 4096 / (int)dv);
   const uint64_t zero_blocks = accumulate ? 0 : ceil_div(vocab, zero_rows);
@@ -476,7 +481,7 @@ agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids
     AGPU_TRY(after_launch(dev, "embedding_index_kernel"));
     auto sum = accumulate ? embedding_sum_kernel<V, true> : embedding_sum_kernel<V, false>;
     AGPU_CUDA(launch_after(sum, sum_blocks + zero_blocks, kThreads, 0, s, g, order, sorted, starts,
-                           d, partial, vocab, own, (int)dv, (int)slices, chunk_len,
+                           d, partial, vocab, own, (int)dv, (int)slices, lanes, chunk_len,
                            (long long)sum_blocks, zero_rows, scale));
     AGPU_TRY(after_launch(dev, "embedding_sum_kernel"));
     if (chunks == 1) return AGPU_OK;

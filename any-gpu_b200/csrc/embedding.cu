@@ -39,6 +39,10 @@ __device__ __forceinline__ float4 times(float4 a, float s) {
   return make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
 }
 __device__ __forceinline__ float times(float a, float s) { return a * s; }
+__device__ __forceinline__ float4 pick(bool c, float4 a) {
+  return make_float4(c ? a.x : 0.f, c ? a.y : 0.f, c ? a.z : 0.f, c ? a.w : 0.f);
+}
+__device__ __forceinline__ float pick(bool c, float a) { return c ? a : 0.f; }
 __device__ __forceinline__ float4 plus(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
@@ -121,10 +125,9 @@ __global__ void __launch_bounds__(kThreads)
       V g[kInFlight];
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u)
-        if (p + u < p1) g[u] = __ldcs(grad + (long long)list[p + u] * dv + col);
+        g[u] = ptx::load_now(grad + (long long)list[min(p + u, p1 - 1)] * dv + col);
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (p + u < p1) acc = plus(acc, g[u]);
+      for (int u = 0; u < kInFlight; ++u) acc = plus(acc, pick(p + u < p1, g[u]));
     }
     acc = times(acc, scale);
     if (accumulate) acc = plus(*dst, acc);
@@ -174,10 +177,10 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
   for (int i0 = begin + lane; i0 < end; i0 += 32 * kIdsAhead) {
     int id[kIdsAhead];
 #pragma unroll
-    for (int u = 0; u < kIdsAhead; ++u)
-      id[u] = i0 + 32 * u < end ? __ldg(ids + i0 + 32 * u) : -1;
+    for (int u = 0; u < kIdsAhead; ++u) id[u] = ptx::load_now(ids + min(i0 + 32 * u, end - 1));
 #pragma unroll
     for (int u = 0; u < kIdsAhead; ++u) {
+      if (i0 + 32 * u >= end) id[u] = -1;
       const bool live = (unsigned)id[u] < (unsigned)vocab;
       const int owner = id[u] & mask;
       if (live && owner == me) atomicAdd(mine + (id[u] >> own.shift), 1);
@@ -237,12 +240,10 @@ __global__ void __launch_bounds__(kIndexWarps * 32)
   for (int i0 = begin; i0 < end; i0 += 32 * kIdsAhead) {
     int id[kIdsAhead];
 #pragma unroll
-    for (int u = 0; u < kIdsAhead; ++u) {
-      const int i = i0 + 32 * u + lane;
-      id[u] = i < end ? __ldg(ids + i) : -1;
-    }
+    for (int u = 0; u < kIdsAhead; ++u) id[u] = ptx::load_now(ids + min(i0 + 32 * u + lane, end - 1));
 #pragma unroll
     for (int u = 0; u < kIdsAhead; ++u) {
+      if (i0 + 32 * u + lane >= end) id[u] = -1;
       const bool in = (unsigned)id[u] < (unsigned)vocab && (id[u] & mask) == me;
       const unsigned who = __ballot_sync(0xffffffffu, in);
       if (who == 0) continue;
@@ -374,11 +375,12 @@ __global__ void __launch_bounds__(kThreads)
     for (int k = group * per; k < end; k += kInFlight) {
       V part[kInFlight];
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (k + u < end) part[u] = partial[(2 * (chunk + k + u) + (k + u == 0)) * dv + col];
+      for (int u = 0; u < kInFlight; ++u) {
+        const int j = min(k + u, end - 1);
+        part[u] = ptx::load_now(partial + (2 * (chunk + j) + (j == 0)) * dv + col);
+      }
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (k + u < end) acc = plus(acc, part[u]);
+      for (int u = 0; u < kInFlight; ++u) acc = plus(acc, pick(k + u < end, part[u]));
     }
   }
   sums[group][lane] = acc;

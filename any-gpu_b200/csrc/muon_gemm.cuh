@@ -71,6 +71,13 @@ constexpr int kMaxItems = 24, kFewItems = 6;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kXScale = 32768.0f;  // X and A = X X^T
 constexpr float kMScale = 16384.0f;  // a I + b A + c A A
+// What the tensor core's truncation takes from an accumulator on average: half
+// a unit in the last place (0.72 2^-24 of the value) for each of the n MMAs of
+// full size, at partial sums of half the final value: 0.36 n 2^-24, that is
+// 0.7 2^-23 for the n = 4 of a segment (measured: 0.8 to 1.0e-7, alike in every
+// product).  Alike in all elements, such an error is amplified by the
+// iteration; rounded to a factor a float can hold it is put back.
+constexpr float kUntruncate = 1.0f + 0x1p-23f;
 
 // Operands and result of a product, with P = scale * (A B):
 enum class Mode {
@@ -193,11 +200,17 @@ struct Block {
 __device__ __forceinline__ void load_block(Block& b, int lane, const __half* g, int ld,
                                            int rows) {
   g += (long long)(lane >> 3) * ld + (lane & 7) * 8;
+  if (rows >= 32) {  // loads that no condition selects: all in flight at once
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    b.d[i] = make_uint4(0, 0, 0, 0);
-    if (i * 4 + (lane >> 3) < rows)
+    for (int i = 0; i < 8; ++i)
       b.d[i] = *reinterpret_cast<const uint4*>(g + (long long)i * 4 * ld);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      b.d[i] = make_uint4(0, 0, 0, 0);
+      if (i * 4 + (lane >> 3) < rows)
+        b.d[i] = *reinterpret_cast<const uint4*>(g + (long long)i * 4 * ld);
+    }
   }
 }
 
@@ -246,11 +259,17 @@ __device__ __forceinline__ void update_block(const float* v, uint8_t* stg, int l
   if (pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && len >= 32) {
     const int l0 = lane >> 3, p = lane & 7;
     float4 old[8];
+    if (keep && lines >= 32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (keep && i * 4 + l0 < lines)
+      for (int i = 0; i < 8; ++i)
         old[i] = *reinterpret_cast<const float4*>(w + (i * 4 + l0) * pitch + p * 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (keep && i * 4 + l0 < lines)
+          old[i] = *reinterpret_cast<const float4*>(w + (i * 4 + l0) * pitch + p * 4);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

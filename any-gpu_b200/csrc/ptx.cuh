@@ -25,6 +25,34 @@ __device__ __forceinline__ unsigned long long globaltimer() {
   return t;
 }
 
+// Global loads that stay where they are written, so that a batch of them is in
+// flight together: the compiler moves a plain load whose value is used under a
+// condition to that use, and each is then waited for in turn.
+__device__ __forceinline__ float load_now(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 load_now(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int load_now(const int* p) {
+  int v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+// A predicated store: a run of these under differing conditions has no branches.
+__device__ __forceinline__ void store_shared_if(bool on, float* p, float v) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.u32 q, %2, 0; @q st.shared.f32 [%0], %1; }" ::"r"(smem_u32(p)),
+      "f"(v), "r"((uint32_t)on)
+      : "memory");
+}
+
 // Programmatic dependent launch.  griddep_wait blocks until the grid this
 // one was launched after (with the programmatic-serialization attribute) has
 // completed and its memory is visible; a no-op otherwise.  A kernel calls it

@@ -15,7 +15,15 @@ but multiplied by the slope at 0, a = 3.4445, in every later step: by a^5 =
 485 from the initial rounding on.  Rounding X to 22 bits before each step:
 2^-22 (a^5 + a^4 + a^3 + a^2 + a) = 2^-22 685 = 1.6e-4.  An error e of A turns
 a large direction into a dead one, |b| e <= 4.775 2^-20 a step, and the steps
-behind it multiply that by 1 + a + ... + a^4 = 198: 9.0e-4."""
+behind it multiply that by 1 + a + ... + a^4 = 198: 9.0e-4.
+
+SEGMENTS = 3e-4, for groups of wide matrices, whose steps may be taken on A =
+X X^T for up to three steps between two products with X (A' = M A M, M = a I +
+b A + c A^2).  An error e <= 2^-20 of A grows there by at most a^2 = 11.9 a
+step, in directions of small singular values, where M is near a: a segment of
+three moves M by |b| / a (1 + 11.9 + 141) e = 214 e = 2.0e-4, one of two by
+18 e = 1.7e-5.  Later steps do not enlarge a relative error of a small singular
+value.  Of one segment of three and two of two, with TOL: 2.6e-4."""
 from __future__ import annotations
 
 import ctypes as C
@@ -26,6 +34,7 @@ import pytest
 U = 2.0 ** -24
 TOL = 2e-5
 DEGENERATE = 1.1e-3
+SEGMENTS = 3e-4
 A, B, CC = 3.4445, -4.7750, 2.0315
 gpu = pytest.mark.gpu
 
@@ -55,7 +64,8 @@ def _gradient(r, rows, cols):
 
 SHAPES = [(1, 1), (1, 9), (9, 1), (7, 5), (32, 32), (33, 129), (64, 256), (128, 128), (127, 127),
           (130, 100), (129, 257), (256, 512), (200, 1000), (1000, 200), (255, 300), (513, 520),
-          (640, 384), (1024, 1031)]
+          (640, 384), (1024, 1031), (100, 300), (128, 2048), (2000, 64), (40, 513), (1030, 16),
+          (128, 2049), (17, 767), (96, 1500), (65, 256)]
 
 
 @gpu
@@ -81,6 +91,27 @@ def test_batches_and_steps(dev, batch, rows, cols, steps):
     got = dev.read(dev.orthogonalize(dev.upload(x), batch, rows, cols, steps)).reshape(x.shape)
     for g, m in zip(got, x):
         assert _rel(g, _orthogonalize(m, steps)) <= TOL
+
+
+# Groups that fill the card: tiles of CTA pairs, steps on the Gram matrix (m >=
+# 512, n >= 1.5 m), more matrices than a launch takes, of either kind.
+@gpu
+@pytest.mark.parametrize("batch,rows,cols,steps,tol", [
+    (24, 600, 600, 2, TOL), (26, 520, 800, 5, SEGMENTS), (8, 1000, 1537, 4, SEGMENTS),
+    (8, 1537, 1000, 7, SEGMENTS), (7, 1025, 1540, 3, SEGMENTS), (27, 140, 150, 5, TOL),
+    (83, 40, 30, 5, TOL), (50, 20, 600, 3, TOL)])
+def test_large_groups(dev, batch, rows, cols, steps, tol):
+    r = np.random.default_rng(rows)
+    x = np.stack([_gradient(r, rows, cols) for i in range(batch)])
+    X = dev.upload(x)
+    got = dev.read(dev.orthogonalize(X, batch, rows, cols, steps))
+    np.testing.assert_array_equal(got, dev.read(dev.orthogonalize(X, batch, rows, cols, steps)))
+    got = got.reshape(x.shape)
+    few = max(rows, cols) > 256
+    for i in {0, 11, 12, 24, batch - 1} if few else range(batch):
+        if i < batch:
+            assert _rel(got[i], _orthogonalize(x[i], steps)) <= tol
+    assert np.isfinite(got).all()
 
 
 @gpu
@@ -149,6 +180,26 @@ def test_optimizer_steps(dev, nesterov):
             assert np.linalg.norm(got_m - m) <= 4 * U * (np.linalg.norm(m) + np.linalg.norm(g[i]))
         held = [(dev.read(p).reshape(s), dev.read(m).reshape(s))
                 for p, m, s in zip(params, opt.states, shapes)]
+
+
+@gpu
+@pytest.mark.parametrize("small", [2, 40])
+def test_optimizer_steps_over_all_kinds(dev, small):
+    """Wide, square and small matrices in one call, and more small ones than fit
+    beside the others."""
+    from any_gpu import Muon
+    r = np.random.default_rng(small)
+    shapes = [(1024, 1600)] * 8 + [(300, 512), (513, 400)]
+    tiny = [(48, 100), (100, 16), (120, 700)]
+    shapes = (tiny * 20)[:small] + shapes
+    w = [r.standard_normal(s).astype(np.float32) for s in shapes]
+    g = [_gradient(r, *s) for s in shapes]
+    params = [dev.upload(a) for a in w]
+    Muon(lr=0.05).step(dev, params, [dev.upload(a) for a in g], shapes)
+    for i in list(range(min(small, 6))) + [small - 1, small, small + 7, small + 8, small + 9]:
+        want, _, size = _step(w[i], g[i], np.zeros(shapes[i]), 0.05, 0.95, True, 0.01, 5)
+        bound = 4 * U * (np.linalg.norm(want) + size) + (SEGMENTS if i >= small else TOL) * size
+        assert np.linalg.norm(dev.read(params[i]) - want.ravel()) <= bound
 
 
 @gpu

@@ -12,6 +12,7 @@
 // in fixed chunks), so it is deterministic: the tokens are sorted by id first
 // instead of being added with floating-point atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "agpu_internal.cuh"
 #include "ptx.cuh"
@@ -29,7 +30,9 @@ constexpr int kJoinGroups = 4;       // groups of a join CTA, each a part of a r
 constexpr int kMaxChunk = 64;        // sorted positions summed by one CTA, at most
 constexpr int kInFlight = 8;         // gradient rows a thread has in flight
 constexpr int kIdsAhead = 8;         // ids a thread of the index has in flight
-constexpr int kFewTokens = 128;      // tokens of the one-launch gradient, at most
+constexpr int kFewCtas = 4;          // its CTAs on an SM
+constexpr int kFewTokens = 256;      // tokens of the one-launch gradient, at most
+constexpr int kFewRows = 16;         // table rows of one of its CTAs, at most
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -80,40 +83,73 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // -------------------------------------------------------------- gradient --
-// Few tokens: one launch, no scratch.  Each CTA owns `rows` table rows and 256
-// columns, orders the tokens of its rows by (row, position) in shared memory,
-// and writes every element: its sum, or zero.  Bound by launch latency or, for
-// a large table, by the zeros; 37 tokens into 1001 x 99: 6 us, sorting 17.
+// Few tokens and a table of a few MB: one launch, no scratch.  Each CTA owns
+// `rows` table rows and 256 columns, orders the tokens of its rows by (row,
+// position) in shared memory, and writes every element: its sum, or zero.
+// Bound by latency: 37 tokens into 1001 x 99 take 4.7 us, sorting them 13; 200
+// into 1000 x 512 7 and 14.  All 256 tokens on one row are its worst case, 21
+// and 14.  In a table of more rows per CTA the zeros take longer than the
+// sorting path's: 8 tokens into 32000 x 4096 88 and 76.
 template <typename V>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kFewCtas)
     embedding_few_kernel(const V* __restrict__ grad, const int* __restrict__ ids,
                          V* __restrict__ d_table, int tokens, int vocab, int dv, int rows,
                          int slices, bool accumulate, float scale, unsigned int* status) {
-  __shared__ int id[kFewTokens], list[kFewTokens], first[kThreads + 1];
-  const int tid = threadIdx.x;
+  constexpr int kPer = kFewTokens / kThreads;
+  // the CTA's tokens by position: ids and positions; then their order
+  __shared__ int id[kFewTokens], pos[kFewTokens], list[kFewTokens], first[kFewRows + 1];
+  __shared__ int counts[kPer * kThreads / 32];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int lo = blockIdx.x / slices * rows, n = min(rows, vocab - lo);
   const int col = blockIdx.x % slices * kThreads + tid;
-  if (tid < tokens) id[tid] = __ldg(ids + tid);
-  __syncthreads();
-  if (tid < tokens) {
-    const int mine = id[tid];
-    if (blockIdx.x == 0 && (mine < -1 || mine >= vocab))
+  int mine[kPer];
+  unsigned in[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) mine[j] = ptx::load_now(ids + min(j * kThreads + tid, tokens - 1));
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const bool live = j * kThreads + tid < tokens;
+    if (blockIdx.x == 0 && live && (mine[j] < -1 || mine[j] >= vocab))
       atomicCAS(status, 0u, AGPU_BAD_TOKEN_CODE);
-    if (mine >= lo && mine < lo + n) {
-      int rank = 0;
-      for (int u = 0; u < tokens; ++u)
-        rank += id[u] >= lo && (id[u] < mine || (id[u] == mine && u < tid));
-      list[rank] = tid;
+    in[j] = __ballot_sync(0xffffffffu, live && mine[j] >= lo && mine[j] < lo + n);
+    if (lane == 0) counts[j * kThreads / 32 + warp] = __popc(in[j]);
+  }
+  __syncthreads();
+  int found = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w == warp && (in[j] >> lane & 1u)) {
+        const int k = found + __popc(in[j] & ((1u << lane) - 1u));
+        id[k] = mine[j];
+        pos[k] = j * kThreads + tid;
+      }
+      found += counts[j * kThreads / 32 + w];
     }
   }
-  for (int r = tid; r <= n; r += kThreads) {  // tokens of rows before row r, r = 0..n
+  __syncthreads();
+  for (int k = tid; k < found; k += kThreads) {
+    int rank = 0;
+    for (int u = 0; u < found; ++u) rank += id[u] < id[k] || (id[u] == id[k] && u < k);
+    list[rank] = pos[k];
+  }
+  if (tid <= n) {  // tokens of rows before row tid, 0..n <= kFewRows
     int before = 0;
-    for (int u = 0; u < tokens; ++u) before += id[u] >= lo && id[u] < lo + r;
-    first[r] = before;
+    for (int u = 0; u < found; ++u) before += id[u] < lo + tid;
+    first[tid] = before;
   }
   __syncthreads();
   if (col >= dv) return;
   V* dst = d_table + (long long)lo * dv + col;
+  auto add = [&](auto most, V& acc, int p, int p1) {
+    V g[most];
+#pragma unroll
+    for (int u = 0; u < most; ++u)
+      g[u] = ptx::load_now(grad + (long long)list[min(p + u, p1 - 1)] * dv + col);
+#pragma unroll
+    for (int u = 0; u < most; ++u) acc = plus(acc, pick(p + u < p1, g[u]));
+  };
   for (int r = 0; r < n; ++r, dst += dv) {
     const int p0 = first[r], p1 = first[r + 1];
     if (p0 == p1) {
@@ -121,14 +157,10 @@ __global__ void __launch_bounds__(kThreads)
       continue;
     }
     V acc = zero(V());
-    for (int p = p0; p < p1; p += kInFlight) {
-      V g[kInFlight];
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        g[u] = ptx::load_now(grad + (long long)list[min(p + u, p1 - 1)] * dv + col);
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) acc = plus(acc, pick(p + u < p1, g[u]));
-    }
+    int p = p0;
+    for (; p1 - p > kInFlight; p += 2 * kInFlight) 
+      add(std::integral_constant<int, 2 * kInFlight>(), acc, p, p1);
+    if (p < p1) add(std::integral_constant<int, kInFlight>(), acc, p, p1);
     acc = times(acc, scale);
     if (accumulate) acc = plus(*dst, acc);
     __stcs(dst, acc);
@@ -435,13 +467,10 @@ template <typename V>
 agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids, float* d_table,
                      int tokens, int vocab, uint32_t dv, float scale, bool accumulate,
                      cudaStream_t s) {
-  if (tokens <= kFewTokens) {
-    const uint64_t slices = ceil_div(dv, kThreads);
-    const uint64_t per = std::min<uint64_t>(
-        kThreads, std::max<uint64_t>(1, vocab * slices / (8ull * dev->sm_count)));
+  const uint64_t slices = ceil_div(dv, kThreads);
+  const uint64_t per = ceil_div(vocab * slices, (uint64_t)kFewCtas * dev->sm_count);
+  if (tokens <= kFewTokens && per <= kFewRows) {
     const uint64_t blocks = ceil_div(vocab, per) * slices;
-    if (blocks > 0x7fffffffull)
-      return fail(AGPU_ERR_UNSUPPORTED, "embedding_backward: too large");
     embedding_few_kernel<V><<<(unsigned)blocks, kThreads, 0, s>>>(
         reinterpret_cast<const V*>(grad_out), ids, reinterpret_cast<V*>(d_table), tokens, vocab,
         (int)dv, (int)per, (int)slices, accumulate, scale, dev->d_status);
@@ -453,7 +482,6 @@ agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids
     ++own.shift;
   own.rows = (int)ceil_div(vocab, 1ull << own.shift);
   const uint64_t slots = (uint64_t)own.rows << own.shift;
-  const uint64_t slices = ceil_div(dv, kThreads);
   // long chunks leave fewer parts to join, if there are enough of them
   const int chunk_len =
       ceil_div(tokens, kMaxChunk) * slices >= 4ull * dev->sm_count ? kMaxChunk : kMaxChunk / 2;

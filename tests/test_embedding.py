@@ -44,7 +44,8 @@ def _gradient(grad, ids, vocab, scale, start=None):
 
 CASES = [(1, 1, 1), (1, 7, 4), (5, 33, 3), (31, 100, 64), (32, 100, 64), (33, 100, 65),
          (64, 31, 99), (65, 1001, 128), (300, 1000, 256), (1000, 777, 1028), (4097, 5000, 36),
-         (20000, 300, 20), (20, 400000, 4), (128, 310000, 3), (129, 310000, 3)]
+         (20000, 300, 20), (20, 400000, 4), (128, 310000, 3), (129, 310000, 3),
+         (256, 600, 512), (257, 600, 512), (255, 9400, 99)]
 
 
 @gpu

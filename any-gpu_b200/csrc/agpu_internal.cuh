@@ -113,6 +113,24 @@ agpu_status check_device_status(agpu_device* dev);
 
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// Launches a kernel that may start while the one before it in the stream ends
+// (it waits for it with griddepcontrol before it touches memory).
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), uint64_t grid, int block, int smem,
+                         cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // ----------------------------------------------------------- op launchers --
 // Implemented in the kernel translation units; all validate nothing (the
 // C-ABI layer validates) and enqueue on `s`.

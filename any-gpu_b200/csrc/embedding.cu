@@ -426,24 +426,6 @@ __global__ void __launch_bounds__(kThreads)
   *dst = y;
 }
 
-// Launches a kernel that may start while the one before it in the stream ends
-// (it waits for it with griddepcontrol before it touches memory).
-template <typename... Params, typename... Args>
-cudaError_t launch_after(void (*kernel)(Params...), uint64_t grid, int block, int smem,
-                         cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid, 1, 1);
-  cfg.blockDim = dim3(block, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-}
-
 template <typename V>
 agpu_status lookup(agpu_device* dev, const float* table, const int32_t* ids, float* out,
                    uint64_t tokens, uint32_t vocab, uint32_t dv, float scale, cudaStream_t s) {

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads)
   double s = 0.0;
   for (int i = threadIdx.x; i < gridDim.x; i += kThreads)
     s += p.partial[(long long)blockIdx.y * gridDim.x + i];
-  const double inv = muon::kXScale / muon::floored_norm(block_sum(s, red));
+  const float inv = (float)(muon::kXScale / muon::floored_norm(block_sum(s, red)));
   auto value = [&](long long i) {
     const float g = it.grad[i];
     return it.momentum ? update_of(g, it.momentum[i], p.mu, p.nesterov) : g;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < 8; ++j) v[j] = c + j < it.cols ? value(at + j) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)(v[j] * inv);
+      for (int j = 0; j < 8; ++j) v[j] *= inv;
       store_split(v, it.x + r * it.ld + c, it.plane);
     }
     return;
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads)
       u[j] = r < it.rows && c < it.cols ? value((long long)r * it.cols + c) : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) tile[lane][warp + 8 * j] = (float)(u[j] * inv);
+    for (int j = 0; j < 8; ++j) tile[lane][warp + 8 * j] = u[j] * inv;
     __syncthreads();
     const int r = threadIdx.x / 8, c = (threadIdx.x % 8) * 8;
     if (c0 + r < it.m) {
@@ -364,7 +364,10 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
     halves += w[i].halves();
     most = std::max(most, (long long)w[i].src.rows * w[i].src.cols);
   }
-  const int parts = (int)std::max<long long>(1, std::min<long long>(kMaxParts, most / 4096));
+  // CTAs per matrix: two waves over all, at least 4096 elements each
+  const long long waves = 16ll * dev->sm_count / count;
+  const int parts = (int)std::max<long long>(
+      1, std::min<long long>({(long long)kMaxParts, waves, most / 4096}));
   void* scratch = nullptr;
   AGPU_TRY(pool_alloc(dev, halves * sizeof(__half) + (size_t)count * parts * sizeof(double),
                       &scratch, s));

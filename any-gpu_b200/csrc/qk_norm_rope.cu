@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "agpu_internal.cuh"
+#include "ptx.cuh"
 
 namespace agpu {
 
@@ -300,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) qk_vec_kernel(const __grid_co
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (!BACKWARD || !a.partial) return;
+  ptx::griddep_launch_dependents();  // qk_weight_grad_kernel, which waits for all of this one
   // the CTA's sums: groups and warps in order
   float4(*red)[32][4] = reinterpret_cast<float4(*)[32][4]>(dyn);
   __syncthreads();
@@ -385,6 +387,7 @@ __global__ void __launch_bounds__(kThreads) qk_any_kernel(const __grid_constant_
     }
   }
   if (BACKWARD && a.partial) {
+    ptx::griddep_launch_dependents();  // qk_weight_grad_kernel, which waits for all of this one
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * dim; i += kThreads) {
       float v = 0.f;
@@ -403,6 +406,7 @@ __global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const float* __res
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int col = blockIdx.x * 32 + lane;
   float v = 0.f;
+  ptx::griddep_wait();
   if (col < 2 * dim) {
 #pragma unroll 8
     for (int p = warp; p < parts; p += 32) v += partial[(long long)p * 2 * dim + col];
@@ -473,6 +477,13 @@ int split_batches(Args& a, int lanes, int j, int sm_count) {
                                   (long long)kCtas * kWarps * sm_count);
 }
 
+agpu_status sum_weight_grads(agpu_device* dev, const Args& a, int parts, float* dq, float* dk,
+                             cudaStream_t s) {
+  AGPU_CUDA(launch_after(qk_weight_grad_kernel, (2 * a.dim + 31) / 32, 1024, 0, s, a.partial, parts,
+                         a.dim, dq, dk));
+  return after_launch(dev, "qk_weight_grad_kernel");
+}
+
 }  // namespace
 
 agpu_status launch_qk_norm_rope(agpu_device* dev, const agpu_qk_norm_rope& d, const float* q,
@@ -535,9 +546,7 @@ agpu_status launch_qk_norm_rope_backward(agpu_device* dev, const agpu_qk_norm_ro
   }
   agpu_status st = after_launch(dev, "qk_norm_rope_backward");
   if (st == AGPU_OK && scratch) {
-    qk_weight_grad_kernel<<<(2 * a.dim + 31) / 32, 1024, 0, s>>>(a.partial, (int)grid, a.dim,
-                                                                 d_q_weight, d_k_weight);
-    st = after_launch(dev, "qk_weight_grad_kernel");
+    st = sum_weight_grads(dev, a, (int)grid, d_q_weight, d_k_weight, s);
   }
   pool_free(dev, scratch, s);
   return st;

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <iterator>
 #include <utility>
 #include <vector>
 
@@ -126,8 +127,9 @@ agpu_status check_muon(float lr, float momentum, float weight_decay, uint32_t st
   return check_steps(steps, fn);
 }
 
-// Written tensors (parameters and momenta) may not share memory: the matrices
-// of a step are updated side by side.  Also checks each for NULL.
+// Written tensors (parameters and momenta) may share memory neither with each
+// other nor with a gradient: the matrices of a step are updated side by side.
+// Also checks each for NULL.
 agpu_status check_muon_tensors(const agpu_muon_tensor* t, uint32_t count, const char* fn) try {
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   spans.reserve(2 * (size_t)count);
@@ -145,13 +147,25 @@ agpu_status check_muon_tensors(const agpu_muon_tensor* t, uint32_t count, const 
   for (size_t i = 1; i < spans.size(); ++i)
     if (spans[i].first < spans[i - 1].second)
       return fail(AGPU_ERR_INVALID, "%s: two parameters or momenta share memory", fn);
+  for (uint32_t i = 0; i < count; ++i) {
+    const uint64_t n = (uint64_t)t[i].rows * t[i].cols;
+    if (n == 0) continue;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t[i].grad), b = a + n * sizeof(float);
+    // the last span that begins before the gradient's end
+    auto it = std::lower_bound(spans.begin(), spans.end(), std::make_pair(b, (uintptr_t)0));
+    if (it != spans.begin() && std::prev(it)->second > a)
+      return fail(AGPU_ERR_INVALID, "%s: gradient %u shares memory with a parameter or momentum",
+                  fn, i);
+  }
   return AGPU_OK;
 } catch (const std::exception&) {
   return fail(AGPU_ERR_OOM, "%s: out of host memory", fn);
 }
 
-agpu_status check_matrix(uint32_t rows, uint32_t cols, const char* fn) {
-  if (rows > 0x7fffffffu || cols > 0x7fffffffu)
+// Elements stay below 2^40 (more than any device holds), so no product wraps.
+agpu_status check_matrix(uint32_t rows, uint32_t cols, const char* fn, uint32_t batch = 1) {
+  const uint64_t n = (uint64_t)rows * cols, most = 1ull << 40;
+  if (rows > 0x7fffffffu || cols > 0x7fffffffu || n > most || (n && batch > most / n))
     return fail(AGPU_ERR_UNSUPPORTED, "%s: matrix too large", fn);
   return AGPU_OK;
 }
@@ -338,7 +352,7 @@ agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t 
   if (!out) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *out = nullptr;
   AGPU_TRY(check_steps(steps, fn));
-  AGPU_TRY(check_matrix(rows, cols, fn));
+  AGPU_TRY(check_matrix(rows, cols, fn, batch));
   AGPU_TRY(check_len(x, (uint64_t)batch * rows * cols, fn, "x"));
   AGPU_TRY(use_device(dev, fn));
   Owned o;
@@ -353,7 +367,7 @@ agpu_status agpu_launch_orthogonalize(agpu_device* dev, const float* x, float* o
                                       void* stream) {
   const char* fn = "launch_orthogonalize";
   AGPU_TRY(check_steps(steps, fn));
-  AGPU_TRY(check_matrix(rows, cols, fn));
+  AGPU_TRY(check_matrix(rows, cols, fn, batch));
   if ((!x || !out) && (uint64_t)batch * rows * cols)
     return fail(AGPU_ERR_INVALID, "%s: NULL pointer", fn);
   AGPU_TRY(use_device(dev, fn));

@@ -353,7 +353,7 @@ AGPU_API agpu_status agpu_embedding(agpu_device* dev, const agpu_buffer* table,
 /* Its gradient: d_table[v] = scale * the sum of grad_out[t] over the tokens t
  * with id v, [vocab, dim], zero rows for ids that do not occur.  Each row's
  * sum has a fixed order, so the result is deterministic.  Pool scratch of
- * about 8 bytes per token, 4 per table row, and 1/16 of grad_out. */
+ * about 8 bytes per token, 4 per table row, and at most 1/16 of grad_out. */
 AGPU_API agpu_status agpu_embedding_backward(agpu_device* dev, const agpu_buffer* grad_out,
                                              const agpu_buffer* ids, uint64_t tokens,
                                              uint32_t vocab, uint32_t dim, float scale,
@@ -502,8 +502,11 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
  * matrix towards 1: X = x / max(|x|_F, 1e-30), then `steps` times
  *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X
  * (on X^T when rows > cols).  x [batch, rows, cols], each matrix by itself.
- * fp32-level accuracy whatever the precision mode.  steps 1..64, else
- * AGPU_ERR_INVALID. */
+ * fp32-level accuracy whatever the precision mode; a NaN or infinity makes its
+ * matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
+ * the other at most 2048 is worked on chip; other matrices take pool scratch,
+ * in groups of up to 24 matrices and 8 GiB: 8 bytes per element of x and 8 per
+ * element of A (wide matrices in large groups: 20 per element of A). */
 AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t batch,
                                         uint32_t rows, uint32_t cols, uint32_t steps,
                                         agpu_buffer** out);
@@ -513,7 +516,9 @@ AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, 
  *   W <- (1 - lr weight_decay) W - lr 0.2 sqrt(max(rows, cols)) orthogonalize(U)
  * The factor gives an update the root mean square of an AdamW step, so both
  * can share a learning rate.  rows / cols are host arrays; M starts at zero;
- * a length other than rows * cols -> AGPU_ERR_SHAPE. */
+ * a length other than rows * cols -> AGPU_ERR_SHAPE; a parameter or momentum
+ * that shares memory with another one or with a gradient -> AGPU_ERR_INVALID.
+ * Pool scratch as agpu_orthogonalize. */
 AGPU_API agpu_status agpu_muon_step(agpu_device* dev, agpu_buffer* const* params,
                                     const agpu_buffer* const* grads, agpu_buffer* const* momenta,
                                     const uint32_t* rows, const uint32_t* cols, uint32_t count,

@@ -153,6 +153,19 @@ def _step(w, g, m, lr, mu, nesterov, wd, steps):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols", [(40, 300), (300, 40), (200, 140)])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_nonfinite_matrix_stays_alone(dev, rows, cols, value):
+    r = np.random.default_rng(9)
+    x = np.stack([_gradient(r, rows, cols) for _ in range(3)])
+    x[1, rows - 1, 3] = value
+    got = dev.read(dev.orthogonalize(dev.upload(x), 3, rows, cols)).reshape(x.shape)
+    assert np.isnan(got[1]).all()
+    for i in (0, 2):
+        assert _rel(got[i], _orthogonalize(x[i])) <= TOL
+
+
+@gpu
 @pytest.mark.parametrize("nesterov", [True, False])
 def test_optimizer_steps(dev, nesterov):
     """Several steps over matrices of equal and different shapes in one call:
@@ -267,6 +280,7 @@ def test_buffer_layer_refusals(dev):
     assert status(lambda: dev.orthogonalize(dev.upload_i32(np.ones(12, int)), 1, 3, 4)) == 2
     assert status(lambda: Muon(0.1).step(dev, [x], [y], [(3, 5)])) == 1
     assert status(lambda: Muon(0.1).step(dev, [x, x], [y, y], [(3, 4), (3, 4)])) == 2  # twice
+    assert status(lambda: Muon(0.1).step(dev, [x], [x], [(3, 4)])) == 2
     assert status(lambda: Muon(0.1).step(dev, [x], [y, y], [(3, 4)])) == 1
     np.testing.assert_array_equal(dev.read(x), np.ones(12))
 
@@ -290,11 +304,18 @@ def test_launch_layer_refusals():
     share = [(1 << 20, 1 << 30, 1 << 24, 8, 8), ((1 << 20) + 252, 1 << 30, 1 << 25, 8, 8)]
     assert step(tensors=share) == 2 and b"share memory" in lib.agpu_last_error_message()
     assert step(tensors=[(1 << 20, 1 << 30, 1 << 20, 8, 8)]) == 2  # momentum is the parameter
+    for grad in (1 << 20, (1 << 20) + 252, (1 << 20) - 252, (1 << 24) + 8, (1 << 20) - 1024):
+        pair = [(1 << 20, 1 << 30, 1 << 24, 8, 8), (1 << 21, grad, 1 << 25, 32, 32)]
+        assert step(tensors=pair) == 2 and b"gradient 1 shares" in lib.agpu_last_error_message()
+    free = [(1 << 20, 1 << 30, 1 << 24, 8, 8), (1 << 21, (1 << 20) + 256, 1 << 25, 8, 8)]
+    assert step(tensors=free) == 2 and b"NULL device" in lib.agpu_last_error_message()
     assert step() == 2 and b"NULL device" in lib.agpu_last_error_message()
     orth = lambda *a: lib.agpu_launch_orthogonalize(None, *a, None)
     assert orth(p, p, 1, 8, 8, 0) == 2
     assert orth(None, p, 1, 8, 8, 5) == 2 and orth(p, None, 1, 8, 8, 5) == 2
     assert orth(p, p, 1, 2**31, 1, 5) == 7
+    assert orth(p, p, 16, 2**30, 2**30, 5) == 7  # 2^64 elements
+    assert orth(p, p, 2**31, 2**10, 1, 5) == 7
     assert orth(p, p, 1, 8, 8, 5) == 2 and b"NULL device" in lib.agpu_last_error_message()
 
 

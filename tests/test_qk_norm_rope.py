@@ -174,6 +174,49 @@ def test_packed_strides_in_place_on_a_callers_stream(dev, dim, shift):
 
 
 @gpu
+@pytest.mark.parametrize("dim", [64, 50])
+def test_strides_past_32_bits(dev, dim):
+    """Two sequences 2^32 + 64 elements apart, rotated in place, and their gradients."""
+    import torch
+    from any_gpu import QkNormRope
+    case = (2, 3, 2, 0, dim, dim, False)
+    b, s, h, _, d, rot, _ = case
+    x, pos = _inputs(case)
+    far = 2 ** 32 + 64
+    buf = torch.empty(far + s * h * d, device="cuda")
+    views = [buf[i * far:i * far + s * h * d].view(s, h, d) for i in range(b)]
+    near, wide = (h * d, d, s * h * d), (h * d, d, far)
+    W = torch.from_numpy(x["qw"]).cuda()
+
+    def fill(a):
+        for v, y in zip(views, a):
+            v.copy_(torch.from_numpy(y))
+        torch.cuda.synchronize()
+
+    def read():
+        dev.synchronize()
+        return np.stack([v.cpu().numpy() for v in views])
+    zeros = (0, 0, 0)
+    fill(x["q"])
+    shape = QkNormRope(b, s, h, 0, d, rot, 1e-6, 10000.0, wide, zeros, wide, zeros)
+    dev.launch_qk_norm_rope(shape, buf.data_ptr(), 0, W.data_ptr(), 0, 0, buf.data_ptr(), 0)
+    want, tol = _forward(x["q"], x["qw"].astype(np.float64), pos, rot, 1e-6, 10000.0)
+    assert (np.abs(read() - want) <= tol).all()
+    fill(x["gq"])  # gradients far apart, the input near
+    Q, dx = torch.from_numpy(x["q"]).cuda(), torch.empty(x["q"].shape, device="cuda")
+    dw = torch.empty(d, device="cuda")
+    torch.cuda.synchronize()
+    shape = QkNormRope(b, s, h, 0, d, rot, 1e-6, 10000.0, near, zeros, wide, zeros)
+    dev.launch_qk_norm_rope_backward(shape, buf.data_ptr(), 0, Q.data_ptr(), 0, W.data_ptr(), 0, 0,
+                                     dx.data_ptr(), 0, dw.data_ptr(), 0)
+    dev.synchronize()
+    want, tol, want_w, tol_w = _backward(x["q"], x["qw"].astype(np.float64), pos, rot, 1e-6,
+                                         10000.0, x["gq"])
+    assert (np.abs(dx.cpu().numpy() - want) <= tol).all()
+    assert (np.abs(dw.cpu().numpy() - want_w) <= tol_w).all()
+
+
+@gpu
 def test_matches_rmsnorm_then_rope(dev):
     """The fused pass against the two ops it fuses: both are within the bound of the formula."""
     b, s, h, d = 2, 17, 3, 128

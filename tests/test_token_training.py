@@ -243,3 +243,54 @@ def test_llama_layer_with_head_norms(dev, orc):
     act = (torch.nn.functional.silu(gu[:, :, 0]) * gu[:, :, 1]).reshape(T, F)
     want = x2 + act @ w["wd"]
     assert (y.double() - want).norm() <= 1e-4 * want.norm()  # as the layer's other tests in 3xTF32
+
+
+@gpu
+def test_calls_on_two_streams_at_once(dev):
+    """Calls that take scratch, side by side on two streams, give what they give alone."""
+    import torch
+    from any_gpu import QkNormRope, muon_tensors
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    tokens, vocab, dim, shape = 3000, 700, 256, QkNormRope(2, 400, 6, 2, 64)
+    sides = []
+    for _ in range(2):
+        sides.append({"ids": torch.randint(-1, vocab, (tokens,), generator=g, device="cuda",
+                                           dtype=torch.int32),
+                      "grad": rand(tokens, dim), "gq": rand(2, 400, 6, 64),
+                      "gk": rand(2, 400, 2, 64), "q": rand(2, 400, 6, 64),
+                      "k": rand(2, 400, 2, 64), "w": rand(64), "mats": [rand(200, 300), rand(60, 90)]})
+
+    def run(x, stream):
+        """Enqueues one call of each; the outputs, filled beforehand."""
+        h = stream.cuda_stream
+        dev.launch_embedding_backward(x["grad"].data_ptr(), x["ids"].data_ptr(),
+                                      x["o"][0].data_ptr(), tokens, vocab, dim, 1.0, stream=h)
+        dev.launch_qk_norm_rope_backward(
+            shape, x["gq"].data_ptr(), x["gk"].data_ptr(), x["q"].data_ptr(), x["k"].data_ptr(),
+            x["w"].data_ptr(), x["w"].data_ptr(), 0, *[t.data_ptr() for t in x["o"][1:5]], h)
+        dev.launch_muon(muon_tensors([(w.data_ptr(), u.data_ptr(), m.data_ptr(), *u.shape)
+                                      for w, u, m in zip(x["o"][5:7], x["mats"], x["o"][7:9])]),
+                        0.02, 0.9, True, 0.0, 5, h)
+
+    def outputs():
+        return [torch.zeros(s, device="cuda") for s in
+                [(vocab, dim), (2, 400, 6, 64), (2, 400, 2, 64), (64,), (64,), (200, 300), (60, 90),
+                 (200, 300), (60, 90)]]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for together in (False, True):
+        for x in sides:
+            x["o"] = outputs()
+        torch.cuda.synchronize()
+        for _ in range(6):
+            for x, stream in zip(sides, streams):
+                run(x, stream)
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append([x["o"] for x in sides])
+    for alone, beside in zip(*results):
+        for a, b in zip(alone, beside):
+            assert torch.equal(a, b)
+    dev.synchronize()

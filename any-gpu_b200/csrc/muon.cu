@@ -13,6 +13,7 @@
 // per launch: two kernels form the scaled split X, then three products a step
 // (muon_gemm.cuh), the last of which updates W in its epilogue.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <mutex>
@@ -500,17 +501,54 @@ agpu_status run_groups(agpu_device* dev, std::vector<Work>& all, bool on_gram, f
   return AGPU_OK;
 }
 
-// Matrices of at most 128 x 2048, each by a cluster of CTAs in one launch; the
+// Matrices of at most 128 x 4096, each by a cluster of CTAs in one launch; the
 // ones with equally many CTAs together.  Against the grouped products: one 64 x
 // 256 takes 53 us instead of 95, one 128 x 2048 92 instead of 218, forty of
-// them 374 instead of 615, 148 of 128 x 256 132 instead of 1204.
-bool is_small(const Source& s) {
-  return s.m <= muon::kSmallRows && s.n <= muon::kSmallCols * muon::kSmallCluster;
+// them 374 instead of 615, 148 of 128 x 256 132 instead of 1204; clusters of 16:
+// one 28 x 3050 66 instead of 263, one 128 x 4096 104 instead of 339, 24 of them
+// 421 instead of 535.
+void set_cluster(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int count, int cluster,
+                 cudaStream_t s) {
+  cfg = {};
+  cfg.gridDim = dim3((unsigned)(count * cluster), 1, 1);
+  cfg.blockDim = dim3(muon::kSmallThreads, 1, 1);
+  cfg.dynamicSmemBytes = muon::kSmallSmem;
+  cfg.stream = s;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+}
+
+// The largest cluster the device takes: above 8 CTAs that depends on how many
+// SMs its groups have.  Asked once per device.
+agpu_status largest_cluster(agpu_device* dev, int* most) {
+  static std::atomic<int> known[64];
+  std::atomic<int>& k = known[dev->ordinal & 63];
+  *most = k.load(std::memory_order_acquire);
+  if (*most) return AGPU_OK;
+  AGPU_CUDA(cudaFuncSetAttribute(muon::muon_small_kernel,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, muon::kSmallSmem));
+  AGPU_CUDA(cudaFuncSetAttribute(muon::muon_small_kernel,
+                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  int clusters = 0;
+  set_cluster(cfg, attr, 1, muon::kSmallCluster, nullptr);
+  AGPU_CUDA(cudaOccupancyMaxActiveClusters(&clusters, muon::muon_small_kernel, &cfg));
+  *most = clusters ? muon::kSmallCluster : 8;
+  k.store(*most, std::memory_order_release);
+  return AGPU_OK;
+}
+
+bool is_small(const Source& s, int cluster) {
+  return s.m <= muon::kSmallRows && s.n <= muon::kSmallCols * cluster;
 }
 
 agpu_status run_small(agpu_device* dev, const std::vector<Work>& all, float mu, bool nesterov,
                       uint32_t steps, cudaStream_t s) {
-  AGPU_CUDA(set_smem_once<muon::muon_small_kernel>(dev, muon::kSmallSmem));
   muon::SmallItems g = {};
   g.mu = mu;
   g.nesterov = nesterov;
@@ -519,18 +557,9 @@ agpu_status run_small(agpu_device* dev, const std::vector<Work>& all, float mu, 
     int count = 0;
     for (size_t i = 0; i <= all.size(); ++i) {
       if (count == muon::kSmallItems || (i == all.size() && count)) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(count * cluster), 1, 1);
-        cfg.blockDim = dim3(muon::kSmallThreads, 1, 1);
-        cfg.dynamicSmemBytes = muon::kSmallSmem;
-        cfg.stream = s;
+        cudaLaunchConfig_t cfg;
         cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = cluster;
-        attr.val.clusterDim.y = 1;
-        attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        set_cluster(cfg, attr, count, cluster, s);
         AGPU_CUDA(cudaLaunchKernelEx(&cfg, muon::muon_small_kernel, g, cluster, dev->d_status));
         AGPU_TRY(after_launch(dev, "muon_small_kernel"));
         count = 0;
@@ -563,7 +592,9 @@ agpu_status run_all(agpu_device* dev, std::vector<Work>& all, float mu, bool nes
   // launches are made anyway: 1024 x 1024 takes 275 us, with four of 64 x 256
   // 277, and 335 if these go on their own (2048 x 2048 with 128 x 2048: 583, 673).
   std::vector<Work> small, large;
-  for (const Work& t : all) (is_small(t.src) ? small : large).push_back(t);
+  int cluster = 0;
+  AGPU_TRY(largest_cluster(dev, &cluster));
+  for (const Work& t : all) (is_small(t.src, cluster) ? small : large).push_back(t);
   if (large.empty() || all.size() > (size_t)muon::kMaxItems) {
     AGPU_TRY(run_small(dev, small, mu, nesterov, steps, s));
     all.swap(large);

@@ -40,7 +40,7 @@
 namespace agpu {
 namespace muon {
 
-constexpr int kSmallRows = 128, kSmallCols = 256, kSmallCluster = 8;
+constexpr int kSmallRows = 128, kSmallCols = 256, kSmallCluster = 16;
 constexpr int kSmallThreads = 256;
 constexpr int kChunkBytes = 2 * kPlane;                      // a plane pair of 64 columns
 constexpr int kSmallX = kSmallCols / 64 * kChunkBytes;       // 128 KB
@@ -318,17 +318,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
         const int r = (i >> 5) * cluster + rank, p = i & 31;
         if (r >= m || p * 4 >= n_rows) continue;
         const uint32_t at = ptx::smem_u32(square_piece(S, r, p));
-        float4 d[kSmallCluster], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kParts = 8;  // in flight
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int q0 = 0; q0 < cluster; q0 += kParts) {
+          float4 d[kParts];
 #pragma unroll
-        for (int q = 0; q < kSmallCluster; ++q)
-          if (q < cluster)
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(d[q].x), "=f"(d[q].y), "=f"(d[q].z), "=f"(d[q].w)
-                         : "r"(ptx::mapa(at, q)));
+          for (int q = 0; q < kParts; ++q)
+            if (q0 + q < cluster)
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(d[q].x), "=f"(d[q].y), "=f"(d[q].z), "=f"(d[q].w)
+                           : "r"(ptx::mapa(at, q0 + q)));
 #pragma unroll
-        for (int q = 0; q < kSmallCluster; ++q)
-          if (q < cluster)
-            sum = make_float4(sum.x + d[q].x, sum.y + d[q].y, sum.z + d[q].z, sum.w + d[q].w);
+          for (int q = 0; q < kParts; ++q)
+            if (q0 + q < cluster)
+              sum = make_float4(sum.x + d[q].x, sum.y + d[q].y, sum.z + d[q].z, sum.w + d[q].w);
+        }
         for (int q = 0; q < cluster; ++q)
           asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(ptx::mapa(at, q)),
                        "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w)

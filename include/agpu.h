@@ -504,7 +504,7 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
  * (on X^T when rows > cols).  x [batch, rows, cols], each matrix by itself.
  * fp32-level accuracy whatever the precision mode; a NaN or infinity makes its
  * matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
- * the other at most 2048 is worked on chip; other matrices take pool scratch,
+ * the other at most 4096 is worked on chip; other matrices take pool scratch,
  * in groups of up to 24 matrices and 8 GiB: 8 bytes per element of x and 8 per
  * element of A (wide matrices in large groups: 20 per element of A). */
 AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t batch,

@@ -65,7 +65,7 @@ def _gradient(r, rows, cols):
 SHAPES = [(1, 1), (1, 9), (9, 1), (7, 5), (32, 32), (33, 129), (64, 256), (128, 128), (127, 127),
           (130, 100), (129, 257), (256, 512), (200, 1000), (1000, 200), (255, 300), (513, 520),
           (640, 384), (1024, 1031), (100, 300), (128, 2048), (2000, 64), (40, 513), (1030, 16),
-          (128, 2049), (17, 767), (96, 1500), (65, 256)]
+          (128, 2049), (128, 4096), (3900, 60), (19, 4097), (17, 767), (96, 1500), (65, 256)]
 
 
 @gpu

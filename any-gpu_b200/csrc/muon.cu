@@ -11,7 +11,8 @@
 // Matrices whose shorter side is at most 128 go through the whole iteration on
 // chip (muon_small.cuh).  All others of a call go through it together, a group
 // per launch: two kernels form the scaled split X, then three products a step
-// (muon_gemm.cuh), the last of which updates W in its epilogue.
+// (muon_gemm.cuh), the last of which updates W in its epilogue.  A of few long
+// rows is summed from parts over their columns.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -204,6 +205,50 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// A = X X^T of matrices whose columns were dealt out over several items of a
+// launch: the sum of the parts, in order, split again.  Blocks above the
+// diagonal are not stored.
+struct Part {
+  const __half* part;  // the first one; the others follow, 2 planes apart
+  __half* out;
+  long long plane;
+  int m, ld, slices;
+};
+
+struct Parts {
+  Part item[muon::kMaxItems];
+  int blocks;  // CTAs per matrix
+};
+
+__global__ void __launch_bounds__(kThreads) muon_sum_kernel(const __grid_constant__ Parts p) {
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const Part& it = p.item[blockIdx.x / p.blocks];
+  const __half* part = it.part;
+  const long long plane = it.plane;
+  const int groups = it.ld / 8, slices = it.slices, m = it.m;
+  for (int i = blockIdx.x % p.blocks * kThreads + threadIdx.x; i < m * groups;
+       i += p.blocks * kThreads) {
+    const int r = i / groups, c = (i - r * groups) * 8;
+    if (c / muon::kBlock > r / muon::kBlock) continue;
+    const long long at = (long long)r * it.ld + c;
+    float v[8] = {};
+    for (int k = 0; k < slices; ++k) {
+      const uint4 hi = *reinterpret_cast<const uint4*>(part + 2 * k * plane + at);
+      const uint4 lo = *reinterpret_cast<const uint4*>(part + (2 * k + 1) * plane + at);
+      const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&l[j]));
+        v[2 * j] += a.x + b.x;
+        v[2 * j + 1] += a.y + b.y;
+      }
+    }
+    store_split(v, it.out + at, plane);
+  }
+}
+
 // ------------------------------------------------------ tensor-map encode --
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -357,6 +402,29 @@ int segment_length(int steps, int segments, int i) {
   return steps / segments + (i < steps % segments ? 1 : 0);
 }
 
+// K-blocks per item of A = X X^T.  A launch of fewer tiles than SMs takes as long
+// as its longest contraction (256 x 8192: 103 us, where the other products of
+// a step take 14 each), so its columns are dealt out over more items, as short
+// as the SMs and a launch's items allow, but not below 512 columns; the sum of
+// the parts is one more launch.  Five steps on 256 x 8192 take 214 us instead of
+// 592, on 500 x 4000 227 instead of 388, on 300 x 1500 174 instead of 219; below
+// 16 K-blocks saved the launch takes what it gives (300 x 1024).
+int slice_blocks(agpu_device* dev, const Work* w, int count) {
+  constexpr int kLeast = 512 / muon::kBK;
+  int most = 0;
+  for (int i = 0; i < count; ++i) most = std::max(most, (w[i].src.n + muon::kBK - 1) / muon::kBK);
+  for (int len = kLeast; len < most; len += kLeast) {
+    long long tiles = 0, items = 0;
+    for (int i = 0; i < count; ++i) {
+      const int slices = ((w[i].src.n + muon::kBK - 1) / muon::kBK + len - 1) / len;
+      items += slices;
+      tiles += slices * count_tiles(Mode::Gram, w[i].src.m, w[i].src.m, 128);
+    }
+    if (items <= muon::kMaxItems && tiles <= dev->sm_count) return most - len >= 16 ? len : most;
+  }
+  return most;
+}
+
 agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float mu, bool nesterov,
                       uint32_t steps, cudaStream_t s) {
   size_t halves = 0;
@@ -365,6 +433,16 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
     halves += w[i].halves();
     most = std::max(most, (long long)w[i].src.rows * w[i].src.cols);
   }
+  // parts of A of the matrices whose columns are dealt out
+  const int slice = slice_blocks(dev, w, count);
+  auto slices_of = [&](int i) {
+    return ((w[i].src.n + muon::kBK - 1) / muon::kBK + slice - 1) / slice;
+  };
+  Parts sums = {};
+  int summed = 0;
+  for (int i = 0; i < count; ++i)
+    if (slices_of(i) > 1) halves += 2 * (size_t)slices_of(i) * w[i].square;
+  std::vector<CUtensorMap> parts_of[2];  // slices of X, in turn
   // CTAs per matrix: two waves over all, at least 4096 elements each
   const long long waves = 16ll * dev->sm_count / count;
   const int parts = (int)std::max<long long>(
@@ -409,7 +487,20 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
       }
       t.src.x = t.x[0];
       src.item[i] = t.src;
+      const int slices = slices_of(i);
+      if (slices == 1) continue;
+      for (int k = 0; k < 2; ++k)
+        for (int j = 0; j < slices; ++j) {
+          const int c = j * slice * muon::kBK;
+          parts_of[k].emplace_back();
+          AGPU_TRY(make_map(&parts_of[k].back(), t.x[k] + c, m, std::min(slice * muon::kBK, n - c),
+                            t.src.ld, t.src.plane, true));
+        }
+      sums.item[summed++] = {h, t.sq[0].p, t.square, m, t.ld_square, slices};
+      sums.blocks = std::max(sums.blocks, (int)ceil_div((uint64_t)m * t.ld_square / 8, kThreads));
+      h += 2 * (size_t)slices * t.square;
     }
+    sums.blocks = std::min(sums.blocks, 4 * dev->sm_count);
     src.partial = reinterpret_cast<double*>(h);
     const dim3 grid((unsigned)parts, (unsigned)count);
     muon_update_kernel<<<grid, kThreads, 0, s>>>(src);
@@ -426,18 +517,29 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
       constexpr int kGram = 0, kPoly = 3, kPolyGram = 4;
       int total = 1;
       float total_scale = M;
-      g.count = count;
-      for (int i = 0; i < count; ++i) {  // A = X X^T
-        Item& it = g.item[i];
-        it.a = it.b = w[i].xk[cur];
-        it.m = it.n = w[i].src.m;
-        it.k = w[i].src.n;
-        it.out = w[i].sq[kGram].p;
-        it.plane = w[i].square;
-        it.ld = w[i].ld_square;
-        it.scale = T / X;
+      g.count = 0;
+      size_t part = 0;
+      for (int i = 0, sum = 0; i < count; ++i) {  // A = X X^T
+        const int slices = slices_of(i), n = w[i].src.n;
+        for (int j = 0; j < slices; ++j) {
+          Item& it = g.item[g.count++];
+          it.a = it.b = slices > 1 ? parts_of[cur][part++] : w[i].xk[cur];
+          it.m = it.n = w[i].src.m;
+          it.k = slices > 1 ? std::min(slice * muon::kBK, n - j * slice * muon::kBK) : n;
+          it.out = slices > 1 ? const_cast<__half*>(sums.item[sum].part) + 2 * j * w[i].square
+                              : w[i].sq[kGram].p;
+          it.plane = w[i].square;
+          it.ld = w[i].ld_square;
+          it.scale = T / X;
+        }
+        sum += slices > 1;
       }
       AGPU_TRY(product(dev, Mode::Gram, g, s));
+      if (summed) {
+        AGPU_CUDA(launch_after(muon_sum_kernel, (uint64_t)summed * sums.blocks, kThreads, 0, s,
+                               sums));
+        AGPU_TRY(after_launch(dev, "muon_sum_kernel"));
+      }
       for (int j = 0; j < len; ++j) {
         const int poly = j ? kPoly : total;
         g.count = 0;

@@ -506,7 +506,8 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
  * matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
  * the other at most 4096 is worked on chip; other matrices take pool scratch,
  * in groups of up to 24 matrices and 8 GiB: 8 bytes per element of x and 8 per
- * element of A (wide matrices in large groups: 20 per element of A). */
+ * element of A (wide matrices in large groups: 20 per element of A; few wide
+ * ones: 4 more per 512 or more columns). */
 AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t batch,
                                         uint32_t rows, uint32_t cols, uint32_t steps,
                                         agpu_buffer** out);

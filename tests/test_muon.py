@@ -7,7 +7,10 @@ TOL = 2e-5, for matrices whose singular values are spread like a gradient's
 step maps a singular value s to s (a + b l + c l^2), l = s^2 <= 1.46; a relative
 error e of A = X X^T or of B = b A + c A^2 (against its largest eigenvalue)
 moves the result by at most 1.21 (|b| + 2 c 1.46) 1.46 e < 20 e.  The products
-keep 22 bits of each factor and sum in 32-bit accumulators: e <= 2^-20.
+keep 22 bits of each factor and sum in 32-bit accumulators: e <= 2^-20.  (A of a
+long contraction may be a sum of parts P = X' X'^T over columns X' of X, each
+rounded to 22 bits: |P_ij| <= sqrt(P_ii P_jj), and these sum to at most
+sqrt(A_ii A_jj), so the roundings together are within one of that size.)
 
 DEGENERATE = 1.1e-3, for matrices with singular values that stay 0 (rank 1, a
 single entry).  What a step leaves in those directions is not moved towards 1
@@ -65,7 +68,8 @@ def _gradient(r, rows, cols):
 SHAPES = [(1, 1), (1, 9), (9, 1), (7, 5), (32, 32), (33, 129), (64, 256), (128, 128), (127, 127),
           (130, 100), (129, 257), (256, 512), (200, 1000), (1000, 200), (255, 300), (513, 520),
           (640, 384), (1024, 1031), (100, 300), (128, 2048), (2000, 64), (40, 513), (1030, 16),
-          (128, 2049), (128, 4096), (3900, 60), (19, 4097), (17, 767), (96, 1500), (65, 256)]
+          (128, 2049), (128, 4096), (3900, 60), (19, 4097), (17, 767), (96, 1500), (65, 256),
+          (200, 5000), (6000, 140), (300, 1500), (130, 8191), (50, 4200), (260, 1025), (2049, 257)]
 
 
 @gpu
@@ -99,7 +103,8 @@ def test_batches_and_steps(dev, batch, rows, cols, steps):
 @pytest.mark.parametrize("batch,rows,cols,steps,tol", [
     (24, 600, 600, 2, TOL), (26, 520, 800, 5, SEGMENTS), (8, 1000, 1537, 4, SEGMENTS),
     (8, 1537, 1000, 7, SEGMENTS), (7, 1025, 1540, 3, SEGMENTS), (27, 140, 150, 5, TOL),
-    (83, 40, 30, 5, TOL), (50, 20, 600, 3, TOL)])
+    (83, 40, 30, 5, TOL), (50, 20, 600, 3, TOL), (3, 150, 2100, 5, TOL), (9, 5000, 20, 5, TOL),
+    (2, 700, 4000, 5, TOL)])
 def test_large_groups(dev, batch, rows, cols, steps, tol):
     r = np.random.default_rng(rows)
     x = np.stack([_gradient(r, rows, cols) for i in range(batch)])

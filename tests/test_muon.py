@@ -221,12 +221,13 @@ def test_optimizer_steps_over_all_kinds(dev, small):
 
 
 @gpu
-def test_caller_memory_unaligned_stream_and_graph(dev):
+@pytest.mark.parametrize("shapes", [[(50, 77), (128, 128)], [(200, 3001), (300, 260), (60, 70)],
+                                    [(1024, 1540)] * 8])
+def test_caller_memory_unaligned_stream_and_graph(dev, shapes):
     """Odd addresses, a caller's stream, and the same step replayed from two graphs."""
     import torch
     from any_gpu import muon_tensors
     r = np.random.default_rng(2)
-    shapes = [(50, 77), (128, 128)]
     start = [[_gradient(r, *s) for s in shapes] for _ in range(3)]
     results = []
     for mode in ("eager", "graph"):
@@ -257,7 +258,7 @@ def test_caller_memory_unaligned_stream_and_graph(dev):
             assert torch.equal(x, y)
     x = torch.from_numpy(start[0][0]).cuda()
     torch.cuda.synchronize()
-    dev.launch_orthogonalize(x.data_ptr(), x.data_ptr(), 1, 50, 77)  # in place
+    dev.launch_orthogonalize(x.data_ptr(), x.data_ptr(), 1, *shapes[0])  # in place
     dev.synchronize()
     assert _rel(x.cpu().numpy(), _orthogonalize(start[0][0])) <= TOL
 

@@ -41,6 +41,14 @@ agpu_status check_embedding(uint64_t tokens, uint32_t vocab, uint32_t dim, const
   return AGPU_OK;
 }
 
+// The gradient's positions are 32-bit, and its sorting kernel steps up to 256
+// of them past the last token.
+agpu_status check_embedding_backward(uint64_t tokens, uint32_t vocab, uint32_t dim,
+                                     const char* fn) {
+  if (tokens > 0x7fffff00ull) return fail(AGPU_ERR_UNSUPPORTED, "%s: too many tokens", fn);
+  return check_embedding(tokens, vocab, dim, fn);
+}
+
 // Whether no two elements of [batch, seq, heads, dim] share an address: by
 // increasing stride, each axis steps past everything the smaller ones cover.
 bool distinct(const agpu_attn_layout& l, uint32_t batch, uint32_t seq, uint32_t heads,
@@ -197,7 +205,7 @@ agpu_status agpu_embedding_backward(agpu_device* dev, const agpu_buffer* grad_ou
                                     uint32_t dim, float scale, agpu_buffer** d_table) {
   if (!d_table) return fail(AGPU_ERR_INVALID, "embedding_backward: d_table is NULL");
   *d_table = nullptr;
-  AGPU_TRY(check_embedding(tokens, vocab, dim, "embedding_backward"));
+  AGPU_TRY(check_embedding_backward(tokens, vocab, dim, "embedding_backward"));
   AGPU_TRY(check_len(grad_out, tokens * dim, "embedding_backward", "grad_out"));
   AGPU_TRY(check_len(ids, tokens, "embedding_backward", "ids", true));
   AGPU_TRY(use_device(dev, "embedding_backward"));
@@ -225,7 +233,7 @@ agpu_status agpu_launch_embedding_backward(agpu_device* dev, const float* grad_o
                                            const int32_t* ids, float* d_table, uint64_t tokens,
                                            uint32_t vocab, uint32_t dim, float scale,
                                            int accumulate, void* stream) {
-  AGPU_TRY(check_embedding(tokens, vocab, dim, "launch_embedding_backward"));
+  AGPU_TRY(check_embedding_backward(tokens, vocab, dim, "launch_embedding_backward"));
   if (((!grad_out || !ids) && tokens * dim) || (!d_table && (uint64_t)vocab * dim))
     return fail(AGPU_ERR_INVALID, "launch_embedding_backward: NULL pointer");
   AGPU_TRY(use_device(dev, "launch_embedding_backward"));

@@ -30,6 +30,7 @@ constexpr int kJoinGroups = 4;       // groups of a join CTA, each a part of a r
 constexpr int kMaxChunk = 64;        // sorted positions summed by one CTA, at most
 constexpr int kInFlight = 8;         // gradient rows a thread has in flight
 constexpr int kIdsAhead = 8;         // ids a thread of the index has in flight
+static_assert(0x7fffff00ll + 32 * kIdsAhead <= 0x80000000ll, "an int holds every position");
 constexpr int kFewCtas = 4;          // its CTAs on an SM
 constexpr int kFewTokens = 256;      // tokens of the one-launch gradient, at most
 constexpr int kFewRows = 16;         // table rows of one of its CTAs, at most
@@ -180,6 +181,8 @@ __global__ void __launch_bounds__(kThreads, kFewCtas)
 //   order[p] = token position, sorted[p] = its id, for p in sorted order
 //   starts[slot] = first p of the slot of a row (slot_of_row), and behind the
 //   last slot the number of tokens with a row
+// Positions are ints that step up to 32 * kIdsAhead past the last token, and so
+// `tokens` is at most 2^31 - 256 (the caller refuses more).
 // Bound by instruction issue: 4096 tokens 9 us, 65536 28.
 struct Owners {
   int shift, rows;  // owners = 1 << shift, rows of each

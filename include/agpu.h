@@ -352,7 +352,8 @@ AGPU_API agpu_status agpu_embedding(agpu_device* dev, const agpu_buffer* table,
                                     uint32_t dim, float scale, agpu_buffer** out);
 /* Its gradient: d_table[v] = scale * the sum of grad_out[t] over the tokens t
  * with id v, [vocab, dim], zero rows for ids that do not occur.  Each row's
- * sum has a fixed order, so the result is deterministic.  Pool scratch of
+ * sum has a fixed order, so the result is deterministic.  At most 2^31 - 256
+ * tokens (else AGPU_ERR_UNSUPPORTED).  Pool scratch of
  * about 8 bytes per token, 4 per table row, and at most 1/16 of grad_out. */
 AGPU_API agpu_status agpu_embedding_backward(agpu_device* dev, const agpu_buffer* grad_out,
                                              const agpu_buffer* ids, uint64_t tokens,

@@ -273,6 +273,39 @@ def test_launch_layer_refusals():
     assert lib.agpu_upload_i32(None, None, 1, C.byref(out)) == 2
 
 
+def test_most_tokens_of_the_gradient():
+    """The gradient's 32-bit positions hold 2^31 - 256 tokens; the lookup's are 64-bit."""
+    from any_gpu import _lib
+    lib = _lib.load()
+    f, p, out = C.c_float(1), C.c_void_p(256), C.c_void_p()
+    look = lambda n: lib.agpu_launch_embedding(None, p, p, p, n, 5, 1, f, None)
+    back = lambda n: lib.agpu_launch_embedding_backward(None, p, p, p, n, 5, 1, f, 0, None)
+    most = 2**31 - 256
+    assert back(most) == 2 and b"NULL device" in lib.agpu_last_error_message()
+    assert back(most + 1) == 7 and back(2**31 - 32) == 7 and back(2**31 - 1) == 7
+    assert lib.agpu_embedding_backward(None, None, None, most + 1, 5, 1, f, C.byref(out)) == 7
+    assert look(2**31 - 1) == 2 and b"NULL device" in lib.agpu_last_error_message()
+
+
+def test_positions_of_the_sort_stay_in_an_int():
+    """The sorting kernel's position arithmetic in Python integers, for the most tokens
+    the call takes: per warp, the last ids read by the last lane."""
+    warps, ahead, most = 32, 8, 2**31 - 256
+    for tokens in (most, most - 1, most - 31, most - 32 * ahead * warps):
+        assert tokens + warps - 1 < 2**31
+        per = ((tokens + warps - 1) // warps + 31) // 32 * 32
+        end = 0
+        for warp in range(warps):
+            begin, last = end, min(tokens, (warp + 1) * per)
+            assert begin == min(tokens, warp * per) and last >= begin
+            end = last
+            if end > begin:
+                for i0 in (begin + lane + (end - 1 - begin - lane) // (32 * ahead) * 32 * ahead
+                           for lane in range(32) if begin + lane < end):
+                    assert i0 < end and i0 + 32 * ahead < 2**31  # the step behind the last one
+        assert end == tokens
+
+
 def test_formula_against_differences():
     """The gradient the GPU tests compare with, against differences of the lookup (linear)."""
     r = np.random.default_rng(0)

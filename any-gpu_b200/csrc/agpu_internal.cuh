@@ -24,7 +24,8 @@ struct agpu_device {
   // through effective_precision(), which a thread-scoped override shadows
   std::atomic<int> precision{AGPU_PREC_TF32};
   char name[256] = {0};
-  // Device-side status word written by kernels whose bounded waits expire.
+  // Device-side status words (StatusWord); every kernel with bounded waits gets
+  // the first.
   unsigned int* d_status = nullptr;
   std::atomic<uint64_t> launches{0};
   // One reference held by the handle returned from agpu_device_create, one
@@ -108,7 +109,12 @@ cudaError_t set_smem_once(const agpu_device* dev, int bytes) {
   return e;
 }
 
-// Read back and clear the device status word (non-zero = a bounded wait expired).
+// What kernels report, a word each, so that one event does not hide another: the
+// first bounded wait that expired (its code), and ids outside their table.
+enum StatusWord { kWaitStatus, kTokenStatus, kStatusWords };
+
+// Read back the status words and clear the one that is reported: an expired wait
+// before a bad id, which the next call then reports.
 agpu_status check_device_status(agpu_device* dev);
 
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }

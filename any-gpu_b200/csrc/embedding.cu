@@ -6,7 +6,7 @@
 //
 // ids[t] = -1 is padding: a zero row in the lookup, no term in the gradient.
 // Any other id outside [0, vocab) counts as padding too and records
-// AGPU_BAD_TOKEN_CODE in the device status word.
+// AGPU_BAD_TOKEN_CODE in a device status word of its own.
 //
 // The gradient sums each table row's tokens in a fixed order (by position,
 // in fixed chunks), so it is deterministic: the tokens are sorted by id first
@@ -445,10 +445,10 @@ agpu_status lookup(agpu_device* dev, const float* table, const int32_t* ids, flo
   // call is bound by latency and more CTAs with one load each finish sooner
   if (blocks4 >= 8ull * dev->sm_count)
     embedding_kernel<V, 4><<<(unsigned)blocks4, kThreads, 0, s>>>(
-        tb, ids, o, (long long)total, dv, vocab, scale, dev->d_status);
+        tb, ids, o, (long long)total, dv, vocab, scale, dev->d_status + kTokenStatus);
   else
     embedding_kernel<V, 1><<<(unsigned)ceil_div(total, kThreads), kThreads, 0, s>>>(
-        tb, ids, o, (long long)total, dv, vocab, scale, dev->d_status);
+        tb, ids, o, (long long)total, dv, vocab, scale, dev->d_status + kTokenStatus);
   return after_launch(dev, "embedding_kernel");
 }
 
@@ -462,7 +462,7 @@ agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids
     const uint64_t blocks = ceil_div(vocab, per) * slices;
     embedding_few_kernel<V><<<(unsigned)blocks, kThreads, 0, s>>>(
         reinterpret_cast<const V*>(grad_out), ids, reinterpret_cast<V*>(d_table), tokens, vocab,
-        (int)dv, (int)per, (int)slices, accumulate, scale, dev->d_status);
+        (int)dv, (int)per, (int)slices, accumulate, scale, dev->d_status + kTokenStatus);
     return after_launch(dev, "embedding_few_kernel");
   }
   Owners own = {0, 0};
@@ -496,7 +496,7 @@ agpu_status gradient(agpu_device* dev, const float* grad_out, const int32_t* ids
                                                     kIndexWarps * kMaxRowsPerCta * sizeof(int)));
     AGPU_CUDA(launch_after(embedding_index_kernel, 1ull << own.shift, kIndexWarps * 32,
                            kIndexWarps * own.rows * (int)sizeof(int), s, ids, tokens, vocab, own,
-                           order, sorted, starts, dev->d_status));
+                           order, sorted, starts, dev->d_status + kTokenStatus));
     AGPU_TRY(after_launch(dev, "embedding_index_kernel"));
     auto sum = accumulate ? embedding_sum_kernel<V, true> : embedding_sum_kernel<V, false>;
     AGPU_CUDA(launch_after(sum, sum_blocks + zero_blocks, kThreads, 0, s, g, order, sorted, starts,

@@ -100,14 +100,21 @@ agpu_status after_launch(agpu_device* dev, const char* kernel, int n_launches) {
 }
 
 agpu_status check_device_status(agpu_device* dev) {
-  unsigned int h = 0;
-  AGPU_CUDA(cudaMemcpyAsync(&h, dev->d_status, sizeof(h), cudaMemcpyDeviceToHost, dev->stream));
+  unsigned int h[kStatusWords] = {};
+  AGPU_CUDA(cudaMemcpyAsync(h, dev->d_status, sizeof(h), cudaMemcpyDeviceToHost, dev->stream));
   AGPU_CUDA(cudaStreamSynchronize(dev->stream));
-  if (h != 0) {
-    AGPU_CUDA(cudaMemsetAsync(dev->d_status, 0, sizeof(unsigned int), dev->stream));
-    if (h == AGPU_BAD_TOKEN_CODE)
-      return fail(AGPU_ERR_INVALID, "a token id was outside its embedding table (code 0x%x)", h);
-    return fail(AGPU_ERR_TIMEOUT, "a device-side bounded wait expired (code 0x%x)", h);
+  auto clear = [&](int word) {
+    return cudaMemsetAsync(dev->d_status + word, 0, sizeof(unsigned int), dev->stream);
+  };
+  if (h[kWaitStatus] != 0) {
+    AGPU_CUDA(clear(kWaitStatus));
+    return fail(AGPU_ERR_TIMEOUT, "a device-side bounded wait expired (code 0x%x)",
+                h[kWaitStatus]);
+  }
+  if (h[kTokenStatus] != 0) {
+    AGPU_CUDA(clear(kTokenStatus));
+    return fail(AGPU_ERR_INVALID, "a token id was outside its embedding table (code 0x%x)",
+                h[kTokenStatus]);
   }
   return AGPU_OK;
 }
@@ -194,14 +201,14 @@ agpu_status agpu_device_create(int ordinal, agpu_device** out) {
   }
   uint64_t threshold = UINT64_MAX;
   cudaMemPoolSetAttribute(d->pool, cudaMemPoolAttrReleaseThreshold, &threshold);
-  e = cudaMalloc(&d->d_status, sizeof(unsigned int));
+  e = cudaMalloc(&d->d_status, kStatusWords * sizeof(unsigned int));
   if (e != cudaSuccess) {
     cudaMemPoolDestroy(d->pool);
     cudaStreamDestroy(d->stream);
     delete d;
     return cuda_status(e, "cudaMalloc(status)");
   }
-  cudaMemset(d->d_status, 0, sizeof(unsigned int));
+  cudaMemset(d->d_status, 0, kStatusWords * sizeof(unsigned int));
   *out = d;
   return AGPU_OK;
 }

@@ -345,7 +345,8 @@ typedef struct agpu_attn_layout {
  * agpu_upload_i32 buffer of `tokens` ids, out [tokens, dim].  id -1 is padding:
  * a zero row.  Ids are checked on the device: any other id outside [0, vocab)
  * counts as padding and the next agpu_synchronize / agpu_read returns
- * AGPU_ERR_INVALID. */
+ * AGPU_ERR_INVALID (after AGPU_ERR_TIMEOUT, if a bounded wait expired as well:
+ * one event a call). */
 #define AGPU_BAD_TOKEN_CODE 0x7091u
 AGPU_API agpu_status agpu_embedding(agpu_device* dev, const agpu_buffer* table,
                                     const agpu_buffer* ids, uint64_t tokens, uint32_t vocab,

@@ -148,6 +148,23 @@ def test_bad_id_is_reported_and_counts_as_padding(dev, bad):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [3, 300])  # one launch, and sorted
+def test_bad_id_does_not_hide_an_expired_wait(dev, tokens):
+    """A bad id before a wait that runs out: both are reported, the wait first."""
+    from any_gpu import AnyGpuError
+    dev.synchronize()
+    ids = dev.upload_i32([7] + [1] * (tokens - 1))
+    dev.embedding(dev.upload(np.ones(40)), ids, tokens, 5, 8)
+    dev.embedding_backward(dev.upload(np.ones(8 * tokens)), ids, tokens, 5, 8)
+    dev.selftest_wait_timeout(300)
+    for status, code in ((6, "0x7e57"), (2, "0x7091")):
+        with pytest.raises(AnyGpuError) as e:
+            dev.synchronize()
+        assert e.value.status == status and code in str(e.value)
+    dev.synchronize()
+
+
+@gpu
 @pytest.mark.parametrize("shift", [1, 2, 4])
 def test_unaligned_pointers_on_a_callers_stream(dev, shift):
     import torch

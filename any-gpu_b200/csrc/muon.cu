@@ -425,41 +425,110 @@ int slice_blocks(agpu_device* dev, const Work* w, int count) {
   return most;
 }
 
-agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float mu, bool nesterov,
-                      uint32_t steps, cudaStream_t s) {
-  size_t halves = 0;
-  long long most = 0;
-  for (int i = 0; i < count; ++i) {
-    halves += w[i].halves();
-    most = std::max(most, (long long)w[i].src.rows * w[i].src.cols);
-  }
-  // parts of A of the matrices whose columns are dealt out
-  const int slice = slice_blocks(dev, w, count);
-  auto slices_of = [&](int i) {
-    return ((w[i].src.n + muon::kBK - 1) / muon::kBK + slice - 1) / slice;
-  };
+// Matrices that share launches and scratch.
+struct Batch {
+  Work* w;
+  int count;
+  bool on_gram;
+  int slice;       // K-blocks per item of A = X X^T
+  int parts;       // CTAs per matrix that form X
+  int summed = 0;  // matrices whose columns are dealt out
+  Sources src = {};
   Parts sums = {};
-  int summed = 0;
-  for (int i = 0; i < count; ++i)
-    if (slices_of(i) > 1) halves += 2 * (size_t)slices_of(i) * w[i].square;
   std::vector<CUtensorMap> parts_of[2];  // slices of X, in turn
-  // CTAs per matrix: two waves over all, at least 4096 elements each
-  const long long waves = 16ll * dev->sm_count / count;
-  const int parts = (int)std::max<long long>(
-      1, std::min<long long>({(long long)kMaxParts, waves, most / 4096}));
-  void* scratch = nullptr;
-  AGPU_TRY(pool_alloc(dev, halves * sizeof(__half) + (size_t)count * parts * sizeof(double),
-                      &scratch, s));
+
+  int slices(int i) const {
+    return ((w[i].src.n + muon::kBK - 1) / muon::kBK + slice - 1) / slice;
+  }
+  size_t bytes() const {  // of scratch
+    size_t halves = 0;
+    for (int i = 0; i < count; ++i) {
+      halves += w[i].halves();
+      if (slices(i) > 1) halves += 2 * (size_t)slices(i) * w[i].square;  // parts of A
+    }
+    return halves * sizeof(__half) + (size_t)count * parts * sizeof(double);
+  }
+};
+
+// Matrices of one kind as batches that fit a launch and the scratch limit.
+void plan_batches(agpu_device* dev, std::vector<Work>& all, bool on_gram,
+                  std::vector<Batch>& out) {
+  const size_t limit = on_gram ? muon::kMaxItems / 2 : muon::kMaxItems;
+  for (size_t first = 0; first < all.size();) {
+    size_t halves = all[first].halves(), end = first + 1;
+    while (end < all.size() && end - first < limit &&
+           (halves + all[end].halves()) * sizeof(__half) <= kGroupBytes)
+      halves += all[end++].halves();
+    Batch b;
+    b.w = &all[first];
+    b.count = (int)(end - first);
+    b.on_gram = on_gram;
+    b.slice = slice_blocks(dev, b.w, b.count);
+    // CTAs per matrix: two waves over all, at least 4096 elements each
+    long long most = 0;
+    for (int i = 0; i < b.count; ++i)
+      most = std::max(most, (long long)b.w[i].src.rows * b.w[i].src.cols);
+    const long long waves = 16ll * dev->sm_count / b.count;
+    b.parts = (int)std::max<long long>(
+        1, std::min<long long>({(long long)kMaxParts, waves, most / 4096}));
+    out.push_back(std::move(b));
+    first = end;
+  }
+}
+
+// Lays a batch out in the scratch and encodes its tensor maps.
+agpu_status prepare_batch(agpu_device* dev, Batch& b, void* scratch, float mu, bool nesterov) {
+  Sources& src = b.src;
+  src.mu = mu;
+  src.nesterov = nesterov;
+  __half* h = static_cast<__half*>(scratch);
+  for (int i = 0; i < b.count; ++i) {
+    Work& t = b.w[i];
+    const int m = t.src.m, n = t.src.n;
+    for (int k = 0; k < 2; ++k, h += 2 * t.src.plane) {
+      t.x[k] = h;
+      AGPU_TRY(make_map(&t.xk[k], h, m, n, t.src.ld, t.src.plane, true));
+      AGPU_TRY(make_map(&t.xn[k], h, m, n, t.src.ld, t.src.plane, false));
+    }
+    for (int k = 0; k < t.squares; ++k, h += 2 * t.square) {
+      t.sq[k].p = h;
+      AGPU_TRY(make_map(&t.sq[k].k, h, m, m, t.ld_square, t.square, true));
+      AGPU_TRY(make_map(&t.sq[k].n, h, m, m, t.ld_square, t.square, false));
+    }
+    t.src.x = t.x[0];
+    src.item[i] = t.src;
+    const int slices = b.slices(i), cols = b.slice * muon::kBK;
+    if (slices == 1) continue;
+    for (int k = 0; k < 2; ++k)
+      for (int c = 0; c < n; c += cols) {
+        b.parts_of[k].emplace_back();
+        AGPU_TRY(make_map(&b.parts_of[k].back(), t.x[k] + c, m, std::min(cols, n - c), t.src.ld,
+                          t.src.plane, true));
+      }
+    b.sums.item[b.summed++] = {h, t.sq[0].p, t.square, m, t.ld_square, slices};
+    b.sums.blocks =
+        std::max(b.sums.blocks, (int)ceil_div((uint64_t)m * t.ld_square / 8, kThreads));
+    h += 2 * (size_t)slices * t.square;
+  }
+  b.sums.blocks = std::min(b.sums.blocks, 4 * dev->sm_count);
+  src.partial = reinterpret_cast<double*>(h);
+  return AGPU_OK;
+}
+
+// The launches of a prepared batch.
+agpu_status run_batch(agpu_device* dev, const Batch& b, uint32_t steps, cudaStream_t s) {
+  Work* w = b.w;
+  const int count = b.count;
   constexpr float X = muon::kXScale, M = muon::kMScale, T = muon::kUntruncate;
   Group g = {};
   // dst = scale * (a b) of every matrix's squares, added to g
-  auto add_mul = [&](int dst, int a, int b, float scale) {
+  auto add_mul = [&](int dst, int a, int c, float scale) {
     for (int i = 0; i < count; ++i) {
       Item& it = g.item[g.count++];
       it.a = w[i].sq[a].k;
       it.at = w[i].sq[a].n;
-      it.b = w[i].sq[b].k;
-      it.bt = w[i].sq[b].n;
+      it.b = w[i].sq[c].k;
+      it.bt = w[i].sq[c].n;
       it.m = it.n = it.k = w[i].src.m;
       it.out = w[i].sq[dst].p;
       it.plane = w[i].square;
@@ -467,141 +536,94 @@ agpu_status run_group(agpu_device* dev, Work* w, int count, bool on_gram, float 
       it.scale = scale;
     }
   };
-  auto run = [&]() -> agpu_status {
-    Sources src = {};
-    src.mu = mu;
-    src.nesterov = nesterov;
-    __half* h = static_cast<__half*>(scratch);
-    for (int i = 0; i < count; ++i) {
-      Work& t = w[i];
-      const int m = t.src.m, n = t.src.n;
-      for (int k = 0; k < 2; ++k, h += 2 * t.src.plane) {
-        t.x[k] = h;
-        AGPU_TRY(make_map(&t.xk[k], h, m, n, t.src.ld, t.src.plane, true));
-        AGPU_TRY(make_map(&t.xn[k], h, m, n, t.src.ld, t.src.plane, false));
-      }
-      for (int k = 0; k < t.squares; ++k, h += 2 * t.square) {
-        t.sq[k].p = h;
-        AGPU_TRY(make_map(&t.sq[k].k, h, m, m, t.ld_square, t.square, true));
-        AGPU_TRY(make_map(&t.sq[k].n, h, m, m, t.ld_square, t.square, false));
-      }
-      t.src.x = t.x[0];
-      src.item[i] = t.src;
-      const int slices = slices_of(i);
-      if (slices == 1) continue;
-      for (int k = 0; k < 2; ++k)
-        for (int j = 0; j < slices; ++j) {
-          const int c = j * slice * muon::kBK;
-          parts_of[k].emplace_back();
-          AGPU_TRY(make_map(&parts_of[k].back(), t.x[k] + c, m, std::min(slice * muon::kBK, n - c),
-                            t.src.ld, t.src.plane, true));
-        }
-      sums.item[summed++] = {h, t.sq[0].p, t.square, m, t.ld_square, slices};
-      sums.blocks = std::max(sums.blocks, (int)ceil_div((uint64_t)m * t.ld_square / 8, kThreads));
-      h += 2 * (size_t)slices * t.square;
-    }
-    sums.blocks = std::min(sums.blocks, 4 * dev->sm_count);
-    src.partial = reinterpret_cast<double*>(h);
-    const dim3 grid((unsigned)parts, (unsigned)count);
-    muon_update_kernel<<<grid, kThreads, 0, s>>>(src);
-    AGPU_TRY(after_launch(dev, "muon_update_kernel"));
-    muon_split_kernel<<<grid, kThreads, 0, s>>>(src);
-    AGPU_TRY(after_launch(dev, "muon_split_kernel"));
+  const dim3 grid((unsigned)b.parts, (unsigned)count);
+  muon_update_kernel<<<grid, kThreads, 0, s>>>(b.src);
+  AGPU_TRY(after_launch(dev, "muon_update_kernel"));
+  muon_split_kernel<<<grid, kThreads, 0, s>>>(b.src);
+  AGPU_TRY(after_launch(dev, "muon_split_kernel"));
 
-    const int segments =
-        on_gram ? ((int)steps + kMaxSegment - 1) / kMaxSegment : (int)steps;
-    for (int seg = 0; seg < segments; ++seg) {
-      const int len = segment_length((int)steps, segments, seg), cur = seg & 1;
-      // squares: A, the product of the segment's polynomials (in turn), the
-      // step's polynomial, and that times A
-      constexpr int kGram = 0, kPoly = 3, kPolyGram = 4;
-      int total = 1;
-      float total_scale = M;
+  const int segments = b.on_gram ? ((int)steps + kMaxSegment - 1) / kMaxSegment : (int)steps;
+  for (int seg = 0; seg < segments; ++seg) {
+    const int len = segment_length((int)steps, segments, seg), cur = seg & 1;
+    // squares: A, the product of the segment's polynomials (in turn), the
+    // step's polynomial, and that times A
+    constexpr int kGram = 0, kPoly = 3, kPolyGram = 4;
+    int total = 1;
+    float total_scale = M;
+    g.count = 0;
+    size_t part = 0;
+    for (int i = 0, sum = 0; i < count; ++i) {  // A = X X^T
+      const int slices = b.slices(i), n = w[i].src.n;
+      for (int j = 0; j < slices; ++j) {
+        Item& it = g.item[g.count++];
+        it.a = it.b = slices > 1 ? b.parts_of[cur][part++] : w[i].xk[cur];
+        it.m = it.n = w[i].src.m;
+        it.k = slices > 1 ? std::min(b.slice * muon::kBK, n - j * b.slice * muon::kBK) : n;
+        it.out = slices > 1 ? const_cast<__half*>(b.sums.item[sum].part) + 2 * j * w[i].square
+                            : w[i].sq[kGram].p;
+        it.plane = w[i].square;
+        it.ld = w[i].ld_square;
+        it.scale = T / X;
+      }
+      sum += slices > 1;
+    }
+    AGPU_TRY(product(dev, Mode::Gram, g, s));
+    if (b.summed) {
+      AGPU_CUDA(launch_after(muon_sum_kernel, (uint64_t)b.summed * b.sums.blocks, kThreads, 0, s,
+                             b.sums));
+      AGPU_TRY(after_launch(dev, "muon_sum_kernel"));
+    }
+    for (int j = 0; j < len; ++j) {
+      const int poly = j ? kPoly : total;
       g.count = 0;
-      size_t part = 0;
-      for (int i = 0, sum = 0; i < count; ++i) {  // A = X X^T
-        const int slices = slices_of(i), n = w[i].src.n;
-        for (int j = 0; j < slices; ++j) {
-          Item& it = g.item[g.count++];
-          it.a = it.b = slices > 1 ? parts_of[cur][part++] : w[i].xk[cur];
-          it.m = it.n = w[i].src.m;
-          it.k = slices > 1 ? std::min(slice * muon::kBK, n - j * slice * muon::kBK) : n;
-          it.out = slices > 1 ? const_cast<__half*>(sums.item[sum].part) + 2 * j * w[i].square
-                              : w[i].sq[kGram].p;
-          it.plane = w[i].square;
-          it.ld = w[i].ld_square;
-          it.scale = T / X;
-        }
-        sum += slices > 1;
+      add_mul(poly, kGram, kGram, muon::kC * T * (M / (X * X)));
+      for (int i = 0; i < count; ++i) g.item[i].g = w[i].sq[kGram].p;
+      AGPU_TRY(product(dev, Mode::Poly, g, s));
+      g.count = 0;
+      if (j + 1 < len) add_mul(kPolyGram, poly, kGram, T / M);
+      if (j) {
+        const float next = total_scale / 4;  // |polynomial| <= 3.45 a step
+        add_mul(3 - total, poly, total, T * (next / (M * total_scale)));
+        total = 3 - total;
+        total_scale = next;
       }
-      AGPU_TRY(product(dev, Mode::Gram, g, s));
-      if (summed) {
-        AGPU_CUDA(launch_after(muon_sum_kernel, (uint64_t)summed * sums.blocks, kThreads, 0, s,
-                               sums));
-        AGPU_TRY(after_launch(dev, "muon_sum_kernel"));
-      }
-      for (int j = 0; j < len; ++j) {
-        const int poly = j ? kPoly : total;
+      if (g.count) AGPU_TRY(product(dev, Mode::Mul, g, s));
+      if (j + 1 < len) {  // A of the next step
         g.count = 0;
-        add_mul(poly, kGram, kGram, muon::kC * T * (M / (X * X)));
-        for (int i = 0; i < count; ++i) g.item[i].g = w[i].sq[kGram].p;
-        AGPU_TRY(product(dev, Mode::Poly, g, s));
-        g.count = 0;
-        if (j + 1 < len) add_mul(kPolyGram, poly, kGram, T / M);
-        if (j) {
-          const float next = total_scale / 4;  // |polynomial| <= 3.45 a step
-          add_mul(3 - total, poly, total, T * (next / (M * total_scale)));
-          total = 3 - total;
-          total_scale = next;
-        }
-        if (g.count) AGPU_TRY(product(dev, Mode::Mul, g, s));
-        if (j + 1 < len) {  // A of the next step
-          g.count = 0;
-          add_mul(kGram, poly, kPolyGram, T / M);
-          AGPU_TRY(product(dev, Mode::Mul, g, s));
-        }
+        add_mul(kGram, poly, kPolyGram, T / M);
+        AGPU_TRY(product(dev, Mode::Mul, g, s));
       }
-      g.count = count;
-      for (int i = 0; i < count; ++i) {  // times X
-        Item& it = g.item[i];
-        it.a = w[i].sq[total].k;
-        it.at = w[i].sq[total].n;
-        it.bt = w[i].xn[cur];
-        it.m = it.k = w[i].src.m;
-        it.n = w[i].src.n;
-        it.out = w[i].x[1 - cur];
-        it.plane = w[i].src.plane;
-        it.ld = w[i].src.ld;
-        it.scale = T / total_scale;
-        it.w = w[i].w;
-        it.decay = w[i].decay;
-        it.gain = T * (w[i].gain / (X * total_scale));
-        it.w_transposed = w[i].src.rows > w[i].src.cols;
-      }
-      if (seg + 1 < segments) AGPU_TRY(product(dev, Mode::Step, g, s));
-      else AGPU_TRY(product(dev, Mode::Update, g, s));
     }
-    return AGPU_OK;
-  };
-  const agpu_status st = run();
-  pool_free(dev, scratch, s);
-  return st;
-}
-
-// Runs matrices of one kind in groups that fit a launch and the scratch limit.
-agpu_status run_groups(agpu_device* dev, std::vector<Work>& all, bool on_gram, float mu,
-                       bool nesterov, uint32_t steps, cudaStream_t s) {
-  const size_t most = on_gram ? muon::kMaxItems / 2 : muon::kMaxItems;
-  for (size_t first = 0; first < all.size();) {
-    size_t halves = all[first].halves(), end = first + 1;
-    while (end < all.size() && end - first < most &&
-           (halves + all[end].halves()) * sizeof(__half) <= kGroupBytes)
-      halves += all[end++].halves();
-    AGPU_TRY(run_group(dev, &all[first], (int)(end - first), on_gram, mu, nesterov, steps, s));
-    first = end;
+    g.count = count;
+    for (int i = 0; i < count; ++i) {  // times X
+      Item& it = g.item[i];
+      it.a = w[i].sq[total].k;
+      it.at = w[i].sq[total].n;
+      it.bt = w[i].xn[cur];
+      it.m = it.k = w[i].src.m;
+      it.n = w[i].src.n;
+      it.out = w[i].x[1 - cur];
+      it.plane = w[i].src.plane;
+      it.ld = w[i].src.ld;
+      it.scale = T / total_scale;
+      it.w = w[i].w;
+      it.decay = w[i].decay;
+      it.gain = T * (w[i].gain / (X * total_scale));
+      it.w_transposed = w[i].src.rows > w[i].src.cols;
+    }
+    if (seg + 1 < segments) AGPU_TRY(product(dev, Mode::Step, g, s));
+    else AGPU_TRY(product(dev, Mode::Update, g, s));
   }
   return AGPU_OK;
 }
+
+// Scratch of a call, given back when it returns.
+struct Scratch {
+  agpu_device* dev;
+  cudaStream_t s;
+  void* p = nullptr;
+  ~Scratch() { pool_free(dev, p, s); }
+};
 
 // Matrices of at most 128 x 4096, each by a cluster of CTAs in one launch; the
 // ones with equally many CTAs together.  Against the grouped products: one 64 x
@@ -676,7 +698,9 @@ agpu_status run_small(agpu_device* dev, const std::vector<Work>& all, float mu, 
   return AGPU_OK;
 }
 
-// w = decay * w + gain * (orthogonalised update) of every matrix.
+// w = decay * w + gain * (orthogonalised update) of every matrix.  All that can
+// run out (host memory, scratch) is taken before the first launch, as much
+// scratch as the largest batch needs: a call that fails has stepped no matrix.
 agpu_status run_all(agpu_device* dev, std::vector<Work>& all, float mu, bool nesterov,
                     uint32_t steps, cudaStream_t s) {
   for (Work& t : all) {
@@ -697,11 +721,8 @@ agpu_status run_all(agpu_device* dev, std::vector<Work>& all, float mu, bool nes
   int cluster = 0;
   AGPU_TRY(largest_cluster(dev, &cluster));
   for (const Work& t : all) (is_small(t.src, cluster) ? small : large).push_back(t);
-  if (large.empty() || all.size() > (size_t)muon::kMaxItems) {
-    AGPU_TRY(run_small(dev, small, mu, nesterov, steps, s));
-    all.swap(large);
-    if (all.empty()) return AGPU_OK;
-  }
+  if (large.empty() || all.size() > (size_t)muon::kMaxItems) all.swap(large);
+  else small.clear();
   // long contractions first, so that the last wave of a launch is short
   std::stable_sort(all.begin(), all.end(), [](const Work& a, const Work& b) {
     return a.src.m != b.src.m ? a.src.m > b.src.m : a.src.n > b.src.n;
@@ -715,10 +736,22 @@ agpu_status run_all(agpu_device* dev, std::vector<Work>& all, float mu, bool nes
     (is_wide ? wide : rest).push_back(t);
     if (is_wide) pairs += count_tiles(Mode::Gram, t.src.m, t.src.m, 256);
   }
-  if (pairs < dev->sm_count / 2) return run_groups(dev, all, false, mu, nesterov, steps, s);
-  for (Work& t : wide) t.squares = 5;
-  AGPU_TRY(run_groups(dev, wide, true, mu, nesterov, steps, s));
-  return run_groups(dev, rest, false, mu, nesterov, steps, s);
+  std::vector<Batch> batches;
+  if (pairs < dev->sm_count / 2) {
+    plan_batches(dev, all, false, batches);
+  } else {
+    for (Work& t : wide) t.squares = 5;
+    plan_batches(dev, wide, true, batches);
+    plan_batches(dev, rest, false, batches);
+  }
+  size_t bytes = 0;
+  for (const Batch& b : batches) bytes = std::max(bytes, b.bytes());
+  Scratch scratch = {dev, s};
+  if (bytes) AGPU_TRY(pool_alloc(dev, bytes, &scratch.p, s));
+  for (Batch& b : batches) AGPU_TRY(prepare_batch(dev, b, scratch.p, mu, nesterov));
+  AGPU_TRY(run_small(dev, small, mu, nesterov, steps, s));
+  for (const Batch& b : batches) AGPU_TRY(run_batch(dev, b, steps, s));
+  return AGPU_OK;
 }
 
 }  // namespace

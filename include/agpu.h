@@ -521,7 +521,8 @@ AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, 
  * can share a learning rate.  rows / cols are host arrays; M starts at zero;
  * a length other than rows * cols -> AGPU_ERR_SHAPE; a parameter or momentum
  * that shares memory with another one or with a gradient -> AGPU_ERR_INVALID.
- * Pool scratch as agpu_orthogonalize. */
+ * Pool scratch as agpu_orthogonalize, all of it taken before the first launch:
+ * a call that is refused or runs out of memory has stepped no matrix. */
 AGPU_API agpu_status agpu_muon_step(agpu_device* dev, agpu_buffer* const* params,
                                     const agpu_buffer* const* grads, agpu_buffer* const* momenta,
                                     const uint32_t* rows, const uint32_t* cols, uint32_t count,

@@ -264,6 +264,29 @@ def test_caller_memory_unaligned_stream_and_graph(dev, shapes):
 
 
 @gpu
+@pytest.mark.parametrize("shapes", [[(40, 30)] * 30, [(1024, 1600)] * 8])
+def test_out_of_memory_steps_no_matrix(dev, shapes):
+    """One matrix more, whose scratch (275 GB) no device has, in the batch behind the
+    others': none of them is touched.  Its addresses are not memory; nothing reads them."""
+    import torch
+    from any_gpu import AnyGpuError, muon_tensors
+    g = torch.Generator(device="cuda").manual_seed(1)
+    p, u, m = ([torch.randn(s, generator=g, device="cuda") for s in shapes] for _ in range(3))
+    held = [t.clone() for t in p + m]
+    far = [(1 << 52, 1 << 53, 1 << 54, 2**17, 2**17)]
+    own = [(a.data_ptr(), b.data_ptr(), c.data_ptr(), *a.shape) for a, b, c in zip(p, u, m)]
+    torch.cuda.synchronize()
+    with pytest.raises(AnyGpuError) as e:
+        dev.launch_muon(muon_tensors(own + far), 0.02)
+    assert e.value.status == 4
+    dev.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(p + m, held))
+    dev.launch_muon(muon_tensors(own), 0.02)
+    dev.synchronize()
+    assert not any(torch.equal(a, b) for a, b in zip(p + m, held))
+
+
+@gpu
 def test_precision_mode_does_not_matter(dev):
     x = dev.upload(_gradient(np.random.default_rng(0), 256, 384))
     want = dev.read(dev.orthogonalize(x, 1, 256, 384))

@@ -33,6 +33,10 @@
 // times X 1,900, the new X 1,000; the way in (loads, norm, first split) 11,000.
 // 128 x 256: 69 us; 32 x 32: 31; 128 x 2048, a cluster of 8, 92, where summing
 // A over the cluster takes 10,000 cycles a step.
+//
+// Every wait is bounded.  Behind one that expired a CTA issues no more MMAs and
+// stores no result, but takes part in the cluster's barriers to the end; the
+// status word says that the matrix is not valid.
 #pragma once
 
 #include "muon_gemm.cuh"
@@ -110,6 +114,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   uint64_t* done = reinterpret_cast<uint64_t*>(red + 9);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* drain = done + 2;
   // [128] diagonal of A at scale kXScale; [128] a + the polynomial's
   float* diag = reinterpret_cast<float*>(red + 32);
   float* coef = diag + kSmallRows;
@@ -127,6 +132,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 
   if (tid == 0) {
     ptx::mbar_init(done, 1);
+    ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     ptx::tc_fence_after();
   };
   auto finish = [&] {  // all threads: wait for the issued MMAs
-    ok = ptx::mbar_wait(done, phase, status, 0x611, abort_flag) && ok;
+    ok = ok && ptx::mbar_wait(done, phase, status, 0x611, abort_flag);
     phase ^= 1;
     ptx::tc_fence_after();
   };
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 #pragma unroll 1
   for (int step = 0; step < g.steps; ++step) {
     ready();
-    if (tid == 0) {
+    if (tid == 0 && ok && !*abort_flag) {
       const uint32_t idesc = ptx::make_idesc_f16(128, n_rows, false, false);
       for (int pass = 0; pass < 2; ++pass)
         for (int c = 0; c < chunks; ++c) {
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     if (has_diag) diag[row] = d_row;
     ready();
     const int ks = (m + 15) / 16;  // K in 16s of the products with a square
-    if (tid == 0) {
+    if (tid == 0 && ok && !*abort_flag) {
       const uint32_t idesc = ptx::make_idesc_f16(128, n_rows, false, false);
       for (int pass = 0; pass < 2; ++pass)
         for (int k = 0; k < ks; ++k) {
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
       if (has_diag) coef[row] = kA + d_row * (1.0f / kMScale);
     }
     ready();
-    if (tid == 0) {
+    if (tid == 0 && ok && !*abort_flag) {
       // X as an MN-major operand: 64-column chunks kChunkBytes apart, 16 rows of K 2 KB
       const uint32_t idesc = ptx::make_idesc_f16(128, max(chunks, 1) * 64, false, true);
       auto rows_of = [&](uint32_t addr) { return ptx::make_sdesc(addr, kChunkBytes, 1024, 2); };
@@ -456,6 +462,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
         for (int i = 0; i < 32; ++i)
           v[i] = fmaf(ci, __uint_as_float(x[i]), __uint_as_float(y[i]) * (kUntruncate / kMScale));
         if (last) {
+          if (!__all_sync(0xffffffffu, ok)) break;
           const int r0 = (warp & 3) * 32;
           update_block(v, stg, lane, it.w + slice + (tall ? c * pitch + r0 : r0 * pitch + c), pitch,
                        tall, decay, gain, m - r0, w - c);
@@ -467,8 +474,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
       ptx::tmem_wait_st();
     }
   }
-  (void)ok;  // an expired wait is in the status word, and the ones behind it return at once
-
+  if (tid == 0 && (!ok || *abort_flag)) {  // what was issued is behind it before tensor memory is given back
+    ptx::mma_commit(drain);
+    ptx::mbar_wait(drain, 0, status, 0x612, nullptr);
+  }
   ptx::tc_fence_before();
   if (cluster > 1) ptx::cluster_sync();  // no CTA leaves while others may read its memory
   else __syncthreads();

@@ -348,6 +348,20 @@ def test_launch_layer_refusals():
     assert orth(p, p, 1, 8, 8, 5) == 2 and b"NULL device" in lib.agpu_last_error_message()
 
 
+def test_outcomes_of_bounded_waits_are_used():
+    """No kernel goes on as if a wait had succeeded: a statement that drops the outcome of
+    mbar_wait may only be a drain (no abort flag), and none that was collected is dropped.
+    By the source, since no call makes a tensor core stop."""
+    from pathlib import Path
+    import re
+    csrc = Path(__file__).resolve().parents[1] / "any-gpu_b200" / "csrc"
+    text = (csrc / "muon_small.cuh").read_text() + (csrc / "muon_gemm.cuh").read_text()
+    dropped = re.findall(r"[;{})]\s*ptx::mbar_wait\w*(?:<\w+>)?\(([^;]*)\);", text)
+    assert dropped and all(d.split(",")[-1].strip() == "nullptr" for d in dropped), dropped
+    assert "(void)ok" not in text
+    assert re.search(r"if \(!__all_sync\(0xffffffffu, ok\)\) break;[^}]*update_block", text)
+
+
 def test_iteration_of_the_reference():
     """The float64 iteration the GPU tests compare with, against its closed form on the
     singular values."""

@@ -206,10 +206,10 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // A = X X^T of matrices whose columns were dealt out over several items of a
-// launch: the sum of the parts, in order, split again.  Blocks above the
-// diagonal are not stored.
+// launch: the sum of the parts (floats in two planes of halves), in order, split.
+// Blocks above the diagonal are not stored.
 struct Part {
-  const __half* part;  // the first one; the others follow, 2 planes apart
+  const __half* part;  // the first one's planes; the others follow, 2 planes apart
   __half* out;
   long long plane;
   int m, ld, slices;
@@ -234,15 +234,16 @@ __global__ void __launch_bounds__(kThreads) muon_sum_kernel(const __grid_constan
     const long long at = (long long)r * it.ld + c;
     float v[8] = {};
     for (int k = 0; k < slices; ++k) {
-      const uint4 hi = *reinterpret_cast<const uint4*>(part + 2 * k * plane + at);
-      const uint4 lo = *reinterpret_cast<const uint4*>(part + (2 * k + 1) * plane + at);
-      const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+      const uint4 upper = *reinterpret_cast<const uint4*>(part + 2 * k * plane + at);
+      const uint4 lower = *reinterpret_cast<const uint4*>(part + (2 * k + 1) * plane + at);
+      const uint32_t h[4] = {upper.x, upper.y, upper.z, upper.w};
+      const uint32_t l[4] = {lower.x, lower.y, lower.z, lower.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&l[j]));
-        v[2 * j] += a.x + b.x;
-        v[2 * j + 1] += a.y + b.y;
+        float x, y;
+        muon::from_halves(h[j], l[j], x, y);
+        v[2 * j] += x;
+        v[2 * j + 1] += y;
       }
     }
     store_split(v, it.out + at, plane);
@@ -534,6 +535,7 @@ agpu_status run_batch(agpu_device* dev, const Batch& b, uint32_t steps, cudaStre
       it.plane = w[i].square;
       it.ld = w[i].ld_square;
       it.scale = scale;
+      it.part = 0;
     }
   };
   const dim3 grid((unsigned)b.parts, (unsigned)count);
@@ -564,6 +566,7 @@ agpu_status run_batch(agpu_device* dev, const Batch& b, uint32_t steps, cudaStre
         it.plane = w[i].square;
         it.ld = w[i].ld_square;
         it.scale = T / X;
+        it.part = slices > 1;
       }
       sum += slices > 1;
     }
@@ -606,6 +609,7 @@ agpu_status run_batch(agpu_device* dev, const Batch& b, uint32_t steps, cudaStre
       it.plane = w[i].src.plane;
       it.ld = w[i].src.ld;
       it.scale = T / total_scale;
+      it.part = 0;
       it.w = w[i].w;
       it.decay = w[i].decay;
       it.gain = T * (w[i].gain / (X * total_scale));

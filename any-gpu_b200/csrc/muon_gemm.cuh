@@ -108,6 +108,7 @@ struct Item {
   float* w;                // [m, n] or, if w_transposed, [n, m]
   float decay, gain;
   int w_transposed;
+  int part;                // out is a part of a sum: floats, not split (as_halves)
 };
 
 template <int CAP>
@@ -163,6 +164,17 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Parts of a sum stay floats: the upper halves of two of them, and the lower
+// halves, packed, in the two planes that hi and lo would take.
+__device__ __forceinline__ void as_halves(float x, float y, uint32_t& upper, uint32_t& lower) {
+  upper = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  lower = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x5410);
+}
+__device__ __forceinline__ void from_halves(uint32_t upper, uint32_t lower, float& x, float& y) {
+  x = __uint_as_float(__byte_perm(lower, upper, 0x5410));
+  y = __uint_as_float(__byte_perm(lower, upper, 0x7632));
 }
 
 // The epilogue takes a warp's 32 rows in blocks of 64 columns, the next one
@@ -403,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = m - row0;
       const __half* src = it.g + at;  // Poly
       float* w = it.w;                // Update
-      const bool tr = it.w_transposed;
+      const bool tr = it.w_transposed, part = it.part;
       const long long pitch = tr ? m : n;
       const float decay = it.decay;
       // what the epilogue reads, a line per lane, into L2 meanwhile
@@ -488,7 +500,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint32_t hi[32], lo[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+          for (int i = 0; i < 32; ++i)
+            if (part) as_halves(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+            else split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
           store_plane(hi, stg, lane, out + c, ld, rows);
           store_plane(lo, stg, lane, out + plane + c, ld, rows);
         }

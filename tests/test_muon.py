@@ -120,6 +120,36 @@ def test_large_groups(dev, batch, rows, cols, steps, tol):
 
 
 @gpu
+def test_parts_of_a_long_contraction_are_summed_in_32_bits(dev):
+    """A = X X^T of two rows of 8192, dealt out over slices of 512 columns, whose first
+    two parts of A_10 are 8390662 and -8390661 units of the last place of a float of
+    their size: what is left, one unit, is lost if a part keeps fewer bits.
+
+    Every number up to A_10 is a whole one that a float holds: |x|^2 = 2^30, so the
+    scaled X is x itself, sums stay below 2^24, and the factor 1 + 2^-23 moves both
+    parts by one unit.  One step, in a column where row 1 is zero: out_1 = M_10 x_0,
+    M_10 = A_10 (b + c (A_00 + A_11)), A_00 + A_11 = 1.  M_10 2^14 = 2.74 2^-16 is kept
+    in steps of 2^-24, within 7.2e-4 of itself."""
+    x = np.zeros((2, 8192))
+    x[:, :511] = 128
+    x[:, 511] = 42, 439
+    x[0, 512:1023], x[1, 512:1023] = 128, -128
+    x[:, 1023] = 103, -179
+    assert [x[0, s:s + 512] @ x[1, s:s + 512] for s in (0, 512)] == [8390662, -8390661]
+    x[0, 1024:3000] = 512
+    free = iter(range(4096, 8192))
+    rest = 2**30 - int((x * x).sum())
+    while rest:  # the remaining squares, in columns where row 0 is zero
+        v = min(512, int(np.sqrt(rest)))
+        x[1, next(free)] = v
+        rest -= v * v
+    assert (x * x).sum() == 2**30 and x[0] @ x[1] == 1
+    got = dev.read(dev.orthogonalize(dev.upload(x.astype(np.float32)), 1, 2, 8192, 1))
+    want = (B + CC) * 2.0**-30 * 512 / 2**15
+    assert (np.abs(got.reshape(2, 8192)[1, 1024:3000] - want) <= 1e-3 * abs(want)).all()
+
+
+@gpu
 def test_singular_values_are_driven_to_one(dev):
     x = np.random.default_rng(5).standard_normal((96, 200)).astype(np.float32)
     s = np.linalg.svd(dev.read(dev.orthogonalize(dev.upload(x), 1, 96, 200)).reshape(96, 200),

@@ -2,17 +2,19 @@
 // fp32-level accuracy, for a group of matrices of any shapes in one launch.
 //
 // Split operands.  Every matrix of the iteration is kept as two fp16 planes,
-// x 2^e = hi + lo with hi = fp16(x 2^e) and lo = fp16(x 2^e - hi): 22 bits of
-// each value in the 4 bytes a float takes.  The iteration bounds its values
-// (|X| <= 1.21, |A| <= 1.46, |a I + b A + c A A| <= 3.45 in the 2-norm, so
-// every entry too), and e is the power of two that brings this bound just
-// below fp16's largest value: the small entries of large matrices stay far
-// above fp16's subnormals.  A product is three MMAs into one fp32 accumulator,
-// lo hi + hi lo + hi hi (lo lo is below 2^-22), at the fp16 rate, twice
-// tf32's: half the time of the 3xTF32 GEMM (umma2_x3_kernel.cuh), which also
-// has to split its operands in a pass of its own.  Here the epilogue that
-// produces a matrix writes it split, so operands go from global memory
-// through TMA to the tensor core as they are.
+// x 2^e = hi + lo 2^-11 with hi = fp16(x 2^e) and lo = fp16((x 2^e - hi) 2^11):
+// 22 bits of each value in the 4 bytes a float takes.  The iteration bounds its
+// values (|X| <= 1.21, |A| <= 1.46, |a I + b A + c A A| <= 3.45 in the 2-norm,
+// so every entry too), and e is the power of two that brings this bound just
+// below fp16's largest value; lo is as large as hi, so both leave fp16's normal
+// range only for entries below 2^-28.  (With lo unscaled that began at 2^-18:
+// rows 1e-5 of the others came out 2e-5 to 1e-4 off, where fp32 keeps 4e-6.)
+// A product is three MMAs into one fp32 accumulator, (lo hi + hi lo) 2^-11 +
+// hi hi, the shift being an operand of the MMA that follows the small terms (lo
+// lo is below 2^-22), at the fp16 rate, twice tf32's: half the time of the
+// 3xTF32 GEMM (umma2_x3_kernel.cuh), which also has to split its operands in a
+// pass of its own.  Here the epilogue that produces a matrix writes it split,
+// so operands go from global memory through TMA to the tensor core as they are.
 //
 // Segments.  The tensor core's fp32 sum truncates, an error that grows with
 // the number of MMAs summed (a K loop of 1024 in the 3xTF32 GEMM's segments of
@@ -58,6 +60,7 @@ namespace muon {
 constexpr int kBlock = 256;      // blocks of a symmetric matrix: whole ones are stored
 constexpr int kBK = 64;          // fp16 elements of K per stage: one 128-byte row
 constexpr int kSeg = 1;          // K-blocks summed by one accumulator
+static_assert(kSeg == 1, "the small terms of an accumulator come before its hi hi");
 constexpr int kStages = 3;
 constexpr int kEpi = 8;          // epilogue warps
 constexpr int kPlane = 128 * 128;          // bytes of one plane of an operand tile
@@ -77,6 +80,7 @@ constexpr int kMaxItems = 24, kFewItems = 6;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kXScale = 32768.0f;  // X and A = X X^T
 constexpr float kMScale = 16384.0f;  // a I + b A + c A A
+constexpr int kLoShift = 11;          // lo = fp16((x - hi) 2^11)
 // What the tensor core's truncation takes from an accumulator on average: half
 // a unit in the last place (0.72 2^-24 of the value) for each of the n MMAs of
 // full size, at partial sums of half the final value: 0.36 n 2^-24, that is
@@ -161,7 +165,16 @@ __device__ __forceinline__ int k_blocks(const Item& it, const Tile& t) {
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  float2 r;  // (x - hi) 2^11, exact, as x 2^11 - hi 2^11 on two floats at once
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 a, a, %6;\n\tfma.rn.f32x2 a, b, %7, a;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x), "f"(y), "f"(f.x), "f"(f.y), "l"(0x4500000045000000ull),
+        "l"(0xc5000000c5000000ull));
+  static_assert(kLoShift == 11, "the constants are 2048 and -2048, twice");
+  const __half2 l = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -484,10 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 64; ++i) v[i] *= scale;
           if (mode == Mode::Poly) {  // small terms first
-            constexpr float f = kB * (kMScale / kXScale);
+            constexpr float f = kB * (kMScale / kXScale), f_lo = f / (1 << kLoShift);
             put_block(next, stg, lane);
             load_block(next, lane, src + c, ld, rows);
-            add_block(v, f, stg, lane);
+            add_block(v, f_lo, stg, lane);
             put_block(next, stg, lane);
             if (c + 64 < NC && col0 + c + 64 < n)
               load_block(next, lane, src + plane + c + 64, ld, rows);
@@ -614,7 +627,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma(a_desc(kk, 0), b_desc(kk, 1), true);
               }
   #pragma unroll
-              for (int kk = 0; kk < kBK / 16; ++kk) mma(a_desc(kk, 0), b_desc(kk, 0), true);
+              for (int kk = 0; kk < kBK / 16; ++kk) {
+                if (kk > 0) mma(a_desc(kk, 0), b_desc(kk, 0), true);
+                else if (PAIR)
+                  ptx::mma_f16_ss_pair_shifted<kLoShift>(d, a_desc(0, 0), b_desc(0, 0), idesc);
+                else
+                  ptx::mma_f16_ss_shifted<kLoShift>(d, a_desc(0, 0), b_desc(0, 0), idesc);
+              }
               if (PAIR) ptx::mma_commit_pair(&empty[stage], 0x3);
               else ptx::mma_commit(&empty[stage]);
               if (++stage == kStages) { stage = 0; phase ^= 1; }

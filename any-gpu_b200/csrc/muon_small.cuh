@@ -18,7 +18,10 @@
 //   distributed shared memory (each CTA sums 1/C of the elements of all and
 //   stores them to all); S = A; A A; S = b A + c A A; times X; X = a X + that.
 // Within an accumulator all small terms (lo hi, hi lo) come first, so only the
-// hi hi products, at most 16, are truncated at full size.
+// hi hi products, at most 16, are truncated at full size.  Here lo = fp16(x 2^e -
+// hi), without the grouped products' shift, which takes 64 x 256 from 57 us to
+// 62: rows far smaller than the others are held by a X in fp32 (rows 1e-6 of
+// the others: 2.2e-6 off at most).
 //
 // Diagonals.  As the singular values near 1, A and the polynomial near multiples
 // of I, and 22 bits of a diagonal element scale its whole row.  So S holds them
@@ -87,6 +90,15 @@ __device__ __forceinline__ float4* slice_piece(uint8_t* x, int r, int p) {
   return reinterpret_cast<float4*>(x + r * 1024 + ((p ^ (r & 7)) << 4));
 }
 
+// hi and lo of two scaled values, packed.
+__device__ __forceinline__ void split_plain(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 // 32 scaled values of a row (columns c0 .. c0 + 31 of a split image) to both planes.
 __device__ __forceinline__ void put_row(uint8_t* image, int row, int c0, const float (&v)[32]) {
   uint8_t* line = image + (c0 >> 6) * kChunkBytes + row * 128;
@@ -94,10 +106,10 @@ __device__ __forceinline__ void put_row(uint8_t* image, int row, int c0, const f
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uint4 hi, lo;
-    split2(v[8 * j + 0], v[8 * j + 1], hi.x, lo.x);
-    split2(v[8 * j + 2], v[8 * j + 3], hi.y, lo.y);
-    split2(v[8 * j + 4], v[8 * j + 5], hi.z, lo.z);
-    split2(v[8 * j + 6], v[8 * j + 7], hi.w, lo.w);
+    split_plain(v[8 * j + 0], v[8 * j + 1], hi.x, lo.x);
+    split_plain(v[8 * j + 2], v[8 * j + 3], hi.y, lo.y);
+    split_plain(v[8 * j + 4], v[8 * j + 5], hi.z, lo.z);
+    split_plain(v[8 * j + 6], v[8 * j + 7], hi.w, lo.w);
     const int at = ((p0 + j) ^ (row & 7)) << 4;
     *reinterpret_cast<uint4*>(line + at) = hi;
     *reinterpret_cast<uint4*>(line + kPlane + at) = lo;

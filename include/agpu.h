@@ -504,8 +504,9 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
  * matrix towards 1: X = x / max(|x|_F, 1e-30), then `steps` times
  *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X
  * (on X^T when rows > cols).  x [batch, rows, cols], each matrix by itself.
- * fp32-level accuracy whatever the precision mode; a NaN or infinity makes its
- * matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
+ * fp32-level accuracy whatever the precision mode, of the matrix and of each of
+ * its lines along the longer side (entries of X and A keep 22 bits down to 2^-28);
+ * a NaN or infinity makes its matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
  * the other at most 4096 is worked on chip; other matrices take pool scratch,
  * in groups of up to 24 matrices and 8 GiB: 8 bytes per element of x and 8 per
  * element of A (wide matrices in large groups: 20 per element of A; few wide

@@ -119,6 +119,34 @@ def test_large_groups(dev, batch, rows, cols, steps, tol):
     assert np.isfinite(got).all()
 
 
+def _worst_line(got, want):
+    """Largest relative error of a line along the longer side."""
+    axis = 1 if want.shape[0] <= want.shape[1] else 0
+    return (np.linalg.norm(got.reshape(want.shape) - want, axis=axis)
+            / np.linalg.norm(want, axis=axis)).max()
+
+
+@gpu
+@pytest.mark.parametrize("batch,rows,cols,tol", [
+    (1, 64, 256, TOL), (1, 256, 64, TOL), (1, 120, 1000, TOL), (1, 300, 700, TOL),
+    (1, 700, 300, TOL), (1, 200, 5000, TOL), (8, 1000, 1537, SEGMENTS)])
+@pytest.mark.parametrize("scale", [1e-4, 1e-6])
+def test_lines_of_very_different_size(dev, batch, rows, cols, tol, scale):
+    """Every fourth line (along the longer side) far smaller than the others: each is as
+    accurate as the matrix.  With X = D Y, D the lines' scales, A = D Y Y^T D, and what
+    is said above of X, A and M holds of row i relative to |Y_i| d_i, and of their entries
+    (i, j) relative to d_i d_j, as long as an entry keeps its 22 bits: down to 2^-28, and
+    these are above 2^-31 (three bits fewer, in one rounding of several)."""
+    r = np.random.default_rng(rows)
+    x = r.standard_normal((batch, rows, cols)).astype(np.float32)
+    lines = x if rows <= cols else x.transpose(0, 2, 1)
+    lines[:, ::4] *= np.float32(scale)
+    lines[:, 5] *= np.float32(1e-3)
+    got = dev.read(dev.orthogonalize(dev.upload(x), batch, rows, cols)).reshape(x.shape)
+    for i in {0, batch - 1}:
+        assert _worst_line(got[i], _orthogonalize(x[i])) <= tol
+
+
 @gpu
 def test_parts_of_a_long_contraction_are_summed_in_32_bits(dev):
     """A = X X^T of two rows of 8192, dealt out over slices of 512 columns, whose first

@@ -5,6 +5,7 @@
 // checks (returned as AGPU_ERR_SHAPE where the reference's `ensure!` returns
 // Err), a freshly allocated output buffer owned by the caller.
 #include <cstdlib>
+#include <initializer_list>
 #include <vector>
 
 #include "agpu_internal.cuh"
@@ -20,9 +21,16 @@ namespace {
       return fail(AGPU_ERR_CUDA, fn ": cannot select device %d", (dev)->ordinal); \
   } while (0)
 
+// Every op here works on floats: an int32 buffer (agpu_upload_i32) is refused.
+#define CHECK_F32(b, fn, name)                                                            \
+  do {                                                                                    \
+    if ((b)->i32) return fail(AGPU_ERR_INVALID, fn ": " name " must be an f32 buffer");   \
+  } while (0)
+
 #define CHECK_BUF(b, fn, name)                                             \
   do {                                                                     \
     if (!(b)) return fail(AGPU_ERR_INVALID, fn ": " name " is NULL");      \
+    CHECK_F32(b, fn, name);                                                \
   } while (0)
 
 #define CHECK_OUT(o, fn)                                                   \
@@ -33,10 +41,17 @@ namespace {
 
 #define CHECK_LEN(b, want, fn, name)                                                      \
   do {                                                                                    \
+    CHECK_F32(b, fn, name);                                                               \
     if ((b)->len != (uint64_t)(want))                                                     \
       return fail(AGPU_ERR_SHAPE, fn ": " name " has %llu elems, expected %llu",          \
                   (unsigned long long)(b)->len, (unsigned long long)(want));              \
   } while (0)
+
+agpu_status check_f32(const char* fn, std::initializer_list<const agpu_buffer*> buffers) {
+  for (const agpu_buffer* b : buffers)
+    if (b->i32) return fail(AGPU_ERR_INVALID, "%s: an operand must be an f32 buffer", fn);
+  return AGPU_OK;
+}
 
 // Allocate `n` floats, run `launch`, free the output again if it failed.
 template <typename F>
@@ -56,6 +71,7 @@ agpu_status unary(agpu_device* dev, const agpu_buffer* a, agpu_buffer** out, Una
                   const char* fn) {
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!a) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {a}));
   if (!out) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *out = nullptr;
   AGPU_CUDA(cudaSetDevice(dev->ordinal));
@@ -68,6 +84,7 @@ agpu_status binary(agpu_device* dev, const agpu_buffer* a, const agpu_buffer* b,
                    agpu_buffer** out, Binary op, const char* fn) {
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!a || !b) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {a, b}));
   if (!out) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *out = nullptr;
   // src/ops/elementwise.rs:189,194,199,231,237,243,249
@@ -356,6 +373,7 @@ static agpu_status group_norm_impl(agpu_device* dev, const agpu_buffer* x,
                                    const char* fn) {
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!x || !gamma || !beta) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {x, gamma, beta}));
   if (!out) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *out = nullptr;
   AGPU_CUDA(cudaSetDevice(dev->ordinal));
@@ -400,6 +418,7 @@ extern "C" agpu_status agpu_group_norm_backward(agpu_device* dev, const agpu_buf
   const char* fn = "group_norm_backward";
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!grad_out || !input || !gamma) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {grad_out, input, gamma}));
   if (!d_input || !d_gamma || !d_beta) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *d_input = *d_gamma = *d_beta = nullptr;
   AGPU_CUDA(cudaSetDevice(dev->ordinal));
@@ -446,6 +465,7 @@ extern "C" agpu_status agpu_adamw_step(agpu_device* dev, agpu_buffer* const* par
   for (uint32_t i = 0; i < count; ++i) {
     if (!params[i] || !grads[i] || !m[i] || !v[i])
       return fail(AGPU_ERR_INVALID, "adamw_step: NULL buffer at index %u", i);
+    AGPU_TRY(check_f32("adamw_step", {params[i], grads[i], m[i], v[i]}));
     // src/optim.rs:95
     if (params[i]->len != grads[i]->len || m[i]->len != params[i]->len ||
         v[i]->len != params[i]->len)
@@ -535,6 +555,7 @@ static agpu_status sdpa_impl(agpu_device* dev, const agpu_buffer* q, const agpu_
                              bool causal, agpu_buffer** out, const char* fn) {
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!q || !k || !v) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {q, k, v}));
   if (!out) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *out = nullptr;
   AGPU_CUDA(cudaSetDevice(dev->ordinal));
@@ -572,6 +593,7 @@ extern "C" agpu_status agpu_sdpa_backward(agpu_device* dev, const agpu_buffer* q
   const char* fn = "sdpa_backward";
   if (!dev) return fail(AGPU_ERR_INVALID, "%s: NULL device", fn);
   if (!q || !k || !v || !grad_out) return fail(AGPU_ERR_INVALID, "%s: input is NULL", fn);
+  AGPU_TRY(check_f32(fn, {q, k, v, grad_out}));
   if (!d_q || !d_k || !d_v) return fail(AGPU_ERR_INVALID, "%s: out is NULL", fn);
   *d_q = *d_k = *d_v = nullptr;
   AGPU_CUDA(cudaSetDevice(dev->ordinal));

@@ -125,7 +125,8 @@ AGPU_API agpu_status agpu_read(agpu_device* dev, const agpu_buffer* buf, float* 
                                uint64_t n);
 /* H2D copy of n int32 values (token ids, positions) into a new buffer of n
  * 4-byte elements.  The ops below that take ids or positions accept only such
- * buffers (else AGPU_ERR_INVALID); agpu_read returns their bytes.  No
+ * buffers, and all other operands only f32 ones (else AGPU_ERR_INVALID);
+ * agpu_read and agpu_write (and their _async forms) copy the bytes.  No
  * counterpart in the reference, whose buffers are all f32. */
 AGPU_API agpu_status agpu_upload_i32(agpu_device* dev, const int32_t* host, uint64_t n,
                                      agpu_buffer** out);

@@ -45,13 +45,15 @@ def _check(status: int) -> None:
 
 
 class GpuBuffer:
-    """Owned device buffer of f32 (reference: `GpuBuffer`, src/device.rs:22-26)."""
+    """Owned device buffer of f32 (reference: `GpuBuffer`, src/device.rs:22-26),
+    or of int32 where `upload_i32` made it."""
 
-    __slots__ = ("_h", "_dev", "len")
+    __slots__ = ("_h", "_dev", "len", "i32")
 
-    def __init__(self, handle: int, dev: "GpuDevice"):
+    def __init__(self, handle: int, dev: "GpuDevice", i32: bool = False):
         self._h = C.c_void_p(handle)
         self._dev = dev
+        self.i32 = i32
         self.len = int(_lib.load().agpu_buffer_len(self._h))
 
     @property
@@ -80,6 +82,15 @@ class GpuBuffer:
 def _f32(data) -> np.ndarray:
     arr = np.ascontiguousarray(np.asarray(data, dtype=np.float32).reshape(-1))
     return arr
+
+
+def _i32(data, fn: str) -> np.ndarray:
+    arr = np.asarray(data)
+    if arr.size and arr.dtype.kind not in "iu":
+        raise TypeError(f"{fn}: expected integers, got {arr.dtype}")
+    if arr.size and (arr.min() < -2**31 or arr.max() >= 2**31):
+        raise OverflowError(f"{fn}: a value does not fit in 32 bits")
+    return np.ascontiguousarray(arr.reshape(-1), dtype=np.int32)
 
 
 def QkNormRope(batch: int, seq: int, q_heads: int, k_heads: int, dim: int, rot_dim=None,
@@ -200,16 +211,11 @@ class GpuDevice:
 
     def upload_i32(self, data) -> GpuBuffer:
         """int32 values (token ids, positions) in a buffer of their own kind."""
-        arr = np.asarray(data)
-        if arr.size and arr.dtype.kind not in "iu":
-            raise TypeError(f"upload_i32: expected integers, got {arr.dtype}")
-        if arr.size and (arr.min() < -2**31 or arr.max() >= 2**31):
-            raise OverflowError("upload_i32: a value does not fit in 32 bits")
-        arr = np.ascontiguousarray(arr.reshape(-1), dtype=np.int32)
+        arr = _i32(data, "upload_i32")
         out = C.c_void_p()
         _check(_lib.load().agpu_upload_i32(self._h, arr.ctypes.data_as(C.c_void_p), arr.size,
                                            C.byref(out)))
-        return GpuBuffer(out.value, self)
+        return GpuBuffer(out.value, self, i32=True)
 
     def alloc(self, n: int) -> GpuBuffer:
         """Reference: `alloc(n)` (src/device.rs:97)."""
@@ -218,15 +224,17 @@ class GpuDevice:
         return GpuBuffer(out.value, self)
 
     def read(self, buf: GpuBuffer, out: Optional[np.ndarray] = None) -> np.ndarray:
-        """Reference: `read(&GpuBuffer) -> Vec<f32>` (src/device.rs:115)."""
+        """Reference: `read(&GpuBuffer) -> Vec<f32>` (src/device.rs:115); int32
+        values of an `upload_i32` buffer."""
         if out is None:
-            out = np.empty(buf.len, dtype=np.float32)
+            out = np.empty(buf.len, dtype=np.int32 if buf.i32 else np.float32)
         _check(_lib.load().agpu_read(self._h, buf.handle, out.ctypes.data_as(C.c_void_p),
                                      out.size))
         return out
 
     def write(self, buf: GpuBuffer, data: np.ndarray) -> None:
-        arr = _f32(data)
+        """New values of the buffer's kind."""
+        arr = _i32(data, "write") if buf.i32 else _f32(data)
         _check(_lib.load().agpu_write(self._h, buf.handle, arr.ctypes.data_as(C.c_void_p),
                                       arr.size))
 

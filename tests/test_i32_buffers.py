@@ -67,6 +67,23 @@ def test_refused_as_floats(dev, name, at):
 
 
 @pytest.mark.gpu
+def test_read_and_write_keep_the_values(dev):
+    """New ids in an existing buffer, and ids read back: integers, not a float's bits."""
+    table, ids = dev.upload(np.arange(12.0)), dev.upload_i32([2, 0])
+    got = dev.read(ids)
+    assert got.dtype == np.int32 and got.tolist() == [2, 0]
+    dev.write(ids, [1, -1])
+    assert dev.read(ids).tolist() == [1, -1]
+    np.testing.assert_array_equal(dev.read(dev.embedding(table, ids, 2, 3, 4)),
+                                  [4, 5, 6, 7, 0, 0, 0, 0])
+    with pytest.raises(TypeError):
+        dev.write(ids, [1.0, 2.0])
+    with pytest.raises(OverflowError):
+        dev.write(ids, [0, 2**31])
+    assert dev.read(ids).tolist() == [1, -1]
+
+
+@pytest.mark.gpu
 def test_refused_by_the_optimisers(dev):
     from any_gpu import AdamW, AnyGpuError, Muon
     ids, x, y = dev.upload_i32([1, 2]), dev.upload([1, 2]), dev.upload([3, 4])

@@ -376,8 +376,11 @@ agpu_status agpu_launch_orthogonalize(agpu_device* dev, const float* x, float* o
   const char* fn = "launch_orthogonalize";
   AGPU_TRY(check_steps(steps, fn));
   AGPU_TRY(check_matrix(rows, cols, fn, batch));
-  if ((!x || !out) && (uint64_t)batch * rows * cols)
-    return fail(AGPU_ERR_INVALID, "%s: NULL pointer", fn);
+  const uint64_t n = (uint64_t)batch * rows * cols;
+  if ((!x || !out) && n) return fail(AGPU_ERR_INVALID, "%s: NULL pointer", fn);
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(out);
+  if (a != b && (a < b ? b - a : a - b) < n * sizeof(float))
+    return fail(AGPU_ERR_INVALID, "%s: out overlaps x", fn);
   AGPU_TRY(use_device(dev, fn));
   return launch_orthogonalize(dev, x, out, batch, rows, cols, steps, pick_stream(dev, stream));
 }

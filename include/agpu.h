@@ -540,7 +540,7 @@ typedef struct agpu_muon_tensor {
 AGPU_API agpu_status agpu_launch_muon(agpu_device* dev, const agpu_muon_tensor* tensors,
                                       uint32_t count, float lr, float momentum, int nesterov,
                                       float weight_decay, uint32_t steps, void* stream);
-/* out may be x itself, but must not overlap it otherwise.  Pool scratch. */
+/* out may be x itself; another overlap -> AGPU_ERR_INVALID.  Pool scratch. */
 AGPU_API agpu_status agpu_launch_orthogonalize(agpu_device* dev, const float* x, float* out,
                                                uint32_t batch, uint32_t rows, uint32_t cols,
                                                uint32_t steps, void* stream);

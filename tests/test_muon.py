@@ -406,6 +406,22 @@ def test_launch_layer_refusals():
     assert orth(p, p, 1, 8, 8, 5) == 2 and b"NULL device" in lib.agpu_last_error_message()
 
 
+def test_orthogonalize_refuses_an_output_across_its_input():
+    """Matrices are worked on side by side: only the same place is safe."""
+    from any_gpu import _lib
+    lib = _lib.load()
+
+    def status(x, out, batch=2):
+        return lib.agpu_launch_orthogonalize(None, C.c_void_p(x), C.c_void_p(out), batch, 8, 8, 5,
+                                             None)
+    x, size = 1 << 20, 2 * 8 * 8 * 4
+    for out in (x + 4, x - 4, x + size // 2, x + size - 4, x - size + 4):
+        assert status(x, out) == 2 and b"overlaps" in lib.agpu_last_error_message()
+    for out in (x, x + size, x - size):
+        assert status(x, out) == 2 and b"NULL device" in lib.agpu_last_error_message()
+    assert status(x, x + 4, 0) == 2 and b"NULL device" in lib.agpu_last_error_message()
+
+
 def test_outcomes_of_bounded_waits_are_used():
     """No kernel goes on as if a wait had succeeded: a statement that drops the outcome of
     mbar_wait may only be a drain (no abort flag), and none that was collected is dropped.

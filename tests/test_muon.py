@@ -177,6 +177,63 @@ def test_parts_of_a_long_contraction_are_summed_in_32_bits(dev):
     assert (np.abs(got.reshape(2, 8192)[1, 1024:3000] - want) <= 1e-3 * abs(want)).all()
 
 
+def _orthogonalize32(u, steps):
+    """The iteration in float32 throughout."""
+    f = np.float32
+    x = u / f(np.linalg.norm(u.astype(np.float64)))
+    tall = u.shape[0] > u.shape[1]
+    x = x.T if tall else x
+    for _ in range(steps):
+        g = x @ x.T
+        x = f(A) * x + (f(B) * g + f(CC) * (g @ g)) @ x
+    assert x.dtype == f
+    return x.T if tall else x
+
+
+@gpu
+@pytest.mark.parametrize("batch,rows,cols,steps", [
+    (26, 520, 800, 5), (8, 1000, 1537, 4), (8, 1537, 1000, 7), (7, 1025, 1540, 3),
+    (13, 600, 4000, 5), (1, 300, 700, 5), (1, 200, 5000, 5), (1, 1024, 1024, 5)])
+def test_as_accurate_as_float32(dev, batch, rows, cols, steps):
+    """Matrices without small singular values: ten times, at most, the error of the same
+    iteration in float32.  What dominates a product here (the diagonal of M = a I + b A +
+    c A A) is one term: float32 rounds it once, 2^-24.  The kernel rounds both operands to
+    22 bits, 2^-23 each, and truncates the term in up to four MMAs, 2^-23 each, one of which
+    the factor 1 + 2^-23 puts back: 5 2^-23 = 10 2^-24.  Both errors then take the same way
+    through the steps.  (13 of 600 x 4000: twelve and one whose columns are dealt out, both
+    in steps on the Gram matrix.)"""
+    r = np.random.default_rng(rows + batch)
+    x = r.standard_normal((batch, rows, cols)).astype(np.float32)
+    got = dev.read(dev.orthogonalize(dev.upload(x), batch, rows, cols, steps)).reshape(x.shape)
+    for i in {0, batch - 1}:
+        want = _orthogonalize(x[i], steps)
+        assert _rel(got[i], want) <= 10 * _rel(_orthogonalize32(x[i], steps), want)
+
+
+@gpu
+def test_degenerate_members_of_a_wide_group(dev):
+    """On the Gram path, beside ordinary ones: a zero matrix, one of rank 1, one with a NaN,
+    one with an infinity.
+
+    Rank 1, as for DEGENERATE: rounding X before each step leaves 1.6e-4.  An error e <=
+    2^-20 of A turns the large direction into a dead one, |b| e; in a segment the next A' =
+    M A M multiplies it by at most 1.2 a = 4.1.  Steps of segments of 3 and 2 leave |b| e
+    (a^4 + 5.1 a^3 + 22.1 a^2 + a + 5.1) = 4.775 621 e = 2.8e-3."""
+    r = np.random.default_rng(4)
+    x = np.stack([_gradient(r, 520, 800) for _ in range(26)])
+    plain = dev.read(dev.orthogonalize(dev.upload(x), *x.shape)).reshape(x.shape)
+    x[1] = 0
+    x[3] = np.outer(np.linspace(-1, 1, 520), np.arange(1, 801))
+    x[12, 519, 7] = np.nan
+    x[25, 0, 799] = np.inf
+    got = dev.read(dev.orthogonalize(dev.upload(x), *x.shape)).reshape(x.shape)
+    assert not got[1].any()
+    assert _rel(got[3], _orthogonalize(x[3])) <= 3e-3
+    assert np.isnan(got[12]).all() and np.isnan(got[25]).all()
+    rest = [i for i in range(26) if i not in (1, 3, 12, 25)]
+    np.testing.assert_array_equal(got[rest], plain[rest])
+
+
 @gpu
 def test_singular_values_are_driven_to_one(dev):
     x = np.random.default_rng(5).standard_normal((96, 200)).astype(np.float32)

@@ -206,6 +206,27 @@ def test_training_step(dev):
 
 
 @gpu
+def test_a_training_step_moves_every_matrix(dev):
+    """The matrices after a step on the tape's gradients against the float64 step on the same
+    gradients: |W error| <= 4 u (|W| + |move|) + 2e-5 |move|, as in the optimiser's tests."""
+    from any_gpu import Muon
+    from test_muon import TOL, U, _step
+    r = np.random.default_rng(2)
+    params, (ids, target) = _params(r), _batch(r)
+    _, grads, tape = _train_step(dev, params, ids, target)
+    names = ["wq", "wk", "wv", "wo"]
+    bufs = {n: dev.upload(params[n]) for n in names}
+    opt = Muon(lr=1e-2)
+    opt.step(dev, [bufs[n] for n in names], [grads[n] for n in names], [(E, E)] * 4)
+    for n in names:
+        g = dev.read(grads[n]).reshape(E, E)
+        want, _, move = _step(params[n], g, np.zeros((E, E)), 1e-2, 0.95, True, 0.01, 5)
+        got = dev.read(bufs[n]).reshape(E, E)
+        assert np.linalg.norm(got - want) <= 4 * U * (np.linalg.norm(want) + move) + TOL * move
+        assert np.linalg.norm(got - params[n]) >= 0.5 * move > 0
+
+
+@gpu
 def test_llama_layer_with_head_norms(dev, orc):
     """The layer with qk_norm against the same layer composed in float64 on its
     attention inputs: the fused pass is the only difference to the layer without."""

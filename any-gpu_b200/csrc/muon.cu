@@ -6,13 +6,14 @@
 //   X = U / max(|U|_F, 1e-30), then `steps` times (rows <= cols; else on X^T)
 //       A = X X^T,  X <- (a I + b A + c A A) X
 //   W <- (1 - lr wd) W - lr 0.2 sqrt(max(rows, cols)) X
-// which drives the singular values of X towards 1.
+// which drives the singular values of X towards 1 (the iteration's coefficients:
+// K. Jordan et al., 2024; the factor of the update: J. Liu et al., 2025).
 //
-// Matrices whose shorter side is at most 128 go through the whole iteration on
-// chip (muon_small.cuh).  All others of a call go through it together, a group
-// per launch: two kernels form the scaled split X, then three products a step
-// (muon_gemm.cuh), the last of which updates W in its epilogue.  A of few long
-// rows is summed from parts over their columns.
+// Matrices of at most 128 x 4096 go through the whole iteration on chip
+// (muon_small.cuh), unless larger ones are in a call of few.  All others of a
+// call go through it together, a group per launch: two kernels form the scaled
+// split X, then three products a step (muon_gemm.cuh), the last of which updates
+// W in its epilogue.  A of few long rows is summed from parts over their columns.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -404,12 +405,13 @@ int segment_length(int steps, int segments, int i) {
 }
 
 // K-blocks per item of A = X X^T.  A launch of fewer tiles than SMs takes as long
-// as its longest contraction (256 x 8192: 103 us, where the other products of
-// a step take 14 each), so its columns are dealt out over more items, as short
-// as the SMs and a launch's items allow, but not below 512 columns; the sum of
-// the parts is one more launch.  Five steps on 256 x 8192 take 214 us instead of
-// 592, on 500 x 4000 227 instead of 388, on 300 x 1500 174 instead of 219; below
-// 16 K-blocks saved the launch takes what it gives (300 x 1024).
+// as its longest contraction (256 x 8192, each launch by itself under ncu: A 103
+// us, the other products of a step 14 each; dealt out, 16 and 12.5 for the sum of
+// the parts), so its columns are dealt out over more items, as short as the SMs
+// and a launch's items allow, but not below 512 columns.  Five steps on 256 x
+// 8192, launches overlapping, take 217 us instead of 600, on 500 x 4000 231
+// instead of 397, on 300 x 1500 174 instead of 223; below 16 K-blocks saved the
+// launch takes what it gives (300 x 1024).
 int slice_blocks(agpu_device* dev, const Work* w, int count) {
   constexpr int kLeast = 512 / muon::kBK;
   int most = 0;
@@ -631,10 +633,10 @@ struct Scratch {
 
 // Matrices of at most 128 x 4096, each by a cluster of CTAs in one launch; the
 // ones with equally many CTAs together.  Against the grouped products: one 64 x
-// 256 takes 53 us instead of 95, one 128 x 2048 92 instead of 218, forty of
-// them 374 instead of 615, 148 of 128 x 256 132 instead of 1204; clusters of 16:
-// one 28 x 3050 66 instead of 263, one 128 x 4096 104 instead of 339, 24 of them
-// 421 instead of 535.
+// 256 takes 53 us instead of 100, one 128 x 2048 95 instead of 150, forty of
+// them 287 instead of 625, 148 of 128 x 256 136 instead of 1290; clusters of 16:
+// one 28 x 3050 68 instead of 138, one 128 x 4096 105 instead of 174, 24 of them
+// 424 instead of 538.
 void set_cluster(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int count, int cluster,
                  cudaStream_t s) {
   cfg = {};

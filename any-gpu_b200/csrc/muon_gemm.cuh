@@ -44,7 +44,8 @@
 // TFLOP/s of MMAs, 0.85 of the measured fp16 rate; products with X (4096 x 45312
 // together) 3.24 ms, 1408.  In a long run the power limit takes the clock to
 // 1.3 GHz.  One wave of small tiles is bound by its ends: seven products of
-// 1024^3 take 37 us, of which 20 are MMAs.
+// 1024^3 take 37 us, of which 20 are MMAs.  The shift of the small terms costs
+// 0.5 to 2.5% of a product.
 //
 // Every wait is bounded as in umma2_kernel.cuh.
 #pragma once
@@ -70,7 +71,9 @@ constexpr int kStaging = 4096;             // bytes per epilogue warp
 constexpr int kSmem = 1024 + kStages * kStage + kEpi * kStaging + 256;
 constexpr int kThreads = 128 + 32 * kEpi;
 // Registers: 168 a thread at launch (384 threads), then 40 for warps 0-3 and
-// 232 for the epilogue: 128 * 40 + 256 * 232 = 384 * 168.
+// 232 for the epilogue: 128 * 40 + 256 * 232 = 384 * 168.  Spills as
+// ptxas reports them: 108 bytes of stores and 184 of loads with pair tiles, 20
+// and 36 with single ones.
 constexpr int kRegsLow = 40, kRegsHigh = 232;
 // Matrices per launch.  They travel as kernel parameters, 640 bytes each;
 // launches of at most kFewItems keep below 4 KB.
@@ -86,7 +89,10 @@ constexpr int kLoShift = 11;          // lo = fp16((x - hi) 2^11)
 // full size, at partial sums of half the final value: 0.36 n 2^-24, that is
 // 0.7 2^-23 for the n = 4 of a segment (measured: 0.8 to 1.0e-7, alike in every
 // product).  Alike in all elements, such an error is amplified by the
-// iteration; rounded to a factor a float can hold it is put back.
+// iteration; rounded to a factor a float can hold it is put back.  It is the
+// average for that n: one dominant term loses more the earlier it comes (0.72
+// 2^-24 for each MMA behind it), and the on-chip kernel, whose accumulators take up to
+// 16, uses the same factor.  What that leaves is 1e-7 of a product.
 constexpr float kUntruncate = 1.0f + 0x1p-23f;
 
 // Operands and result of a product, with P = scale * (A B):

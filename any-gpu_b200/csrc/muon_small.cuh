@@ -1,7 +1,8 @@
 // The whole Newton-Schulz iteration of a matrix of at most 128 rows (of its
 // shorter side) in one kernel: a cluster of CTAs per matrix, each holding 256
 // columns of X on chip for all steps.  Through the grouped products
-// (muon_gemm.cuh) such a matrix costs 17 launches of 5 us, whatever its size.
+// (muon_gemm.cuh) such a matrix costs 17 launches, 85 us for 32 x 32 and 100 for
+// 64 x 256.
 //
 // Shared memory of a CTA: X split in two fp16 planes (128 KB: four chunks of 64
 // columns, each a plane pair of 128 lines of 128 bytes, 128-byte swizzle) and a
@@ -34,7 +35,7 @@
 // clock a step is 12,000 cycles: issuing the 24 MMAs of A 3,200, reading A back
 // 1,400, splitting it into S 1,000, A A 1,400, the polynomial into S 2,200,
 // times X 1,900, the new X 1,000; the way in (loads, norm, first split) 11,000.
-// 128 x 256: 69 us; 32 x 32: 31; 128 x 2048, a cluster of 8, 92, where summing
+// 128 x 256: 66 us; 32 x 32: 35; 128 x 2048, a cluster of 8, 95, where summing
 // A over the cluster takes 10,000 cycles a step.
 //
 // Every wait is bounded.  Behind one that expired a CTA issues no more MMAs and

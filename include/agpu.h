@@ -355,8 +355,9 @@ AGPU_API agpu_status agpu_embedding(agpu_device* dev, const agpu_buffer* table,
 /* Its gradient: d_table[v] = scale * the sum of grad_out[t] over the tokens t
  * with id v, [vocab, dim], zero rows for ids that do not occur.  Each row's
  * sum has a fixed order, so the result is deterministic.  At most 2^31 - 256
- * tokens (else AGPU_ERR_UNSUPPORTED).  Pool scratch of
- * about 8 bytes per token, 4 per table row, and at most 1/16 of grad_out. */
+ * tokens (else AGPU_ERR_UNSUPPORTED).  Pool scratch: 8 bytes per token, 4 per
+ * table row (rounded up to 128 of them, or more), and 2 ceil(tokens / 32) rows of
+ * dim floats at most; none for up to 256 tokens into a small table. */
 AGPU_API agpu_status agpu_embedding_backward(agpu_device* dev, const agpu_buffer* grad_out,
                                              const agpu_buffer* ids, uint64_t tokens,
                                              uint32_t vocab, uint32_t dim, float scale,
@@ -505,13 +506,20 @@ AGPU_API agpu_status agpu_launch_adamw(agpu_device* dev, const agpu_adamw_tensor
  * matrix towards 1: X = x / max(|x|_F, 1e-30), then `steps` times
  *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X
  * (on X^T when rows > cols).  x [batch, rows, cols], each matrix by itself.
- * fp32-level accuracy whatever the precision mode, of the matrix and of each of
- * its lines along the longer side (entries of X and A keep 22 bits down to 2^-28);
- * a NaN or infinity makes its matrix NaN.  steps 1..64, else AGPU_ERR_INVALID.  A side of at most 128 with
- * the other at most 4096 is worked on chip; other matrices take pool scratch,
- * in groups of up to 24 matrices and 8 GiB: 8 bytes per element of x and 8 per
- * element of A (wide matrices in large groups: 20 per element of A; few wide
- * ones: 4 more per 512 or more columns). */
+ * The arithmetic is the same in every precision mode: operands of 22 bits, sums
+ * in fp32.  After five steps the matrix, and each of its lines along the longer
+ * side however small (entries keep their bits down to 2^-28 of |x|_F), is off by
+ * 3e-7 to 9e-6, as with float32 products.  A NaN or infinity makes its matrix
+ * NaN.  steps 1..64, else AGPU_ERR_INVALID.
+ * Scratch: a matrix of at most 128 on one side and 4096 on the other (2048 where
+ * the device has no clusters of 16) is worked on chip and takes none, unless it
+ * is in a call of at most 24 with a larger one.  All others take pool scratch, in
+ * groups of up to 24 matrices and 8 GiB, that of the largest group for the call:
+ * 8 bytes per element of x and 8 per element of A (wide matrices in large groups:
+ * 20 per element of A; few wide ones: 4 more per 512 or more columns).
+ * How a matrix is worked on goes by the whole call (its number of matrices and
+ * their sizes), so its last bits may differ in other company; the same call gives
+ * the same bits. */
 AGPU_API agpu_status agpu_orthogonalize(agpu_device* dev, const agpu_buffer* x, uint32_t batch,
                                         uint32_t rows, uint32_t cols, uint32_t steps,
                                         agpu_buffer** out);

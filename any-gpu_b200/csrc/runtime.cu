@@ -44,6 +44,10 @@ agpu_status pool_alloc(agpu_device* dev, size_t bytes, void** out, cudaStream_t 
   cudaError_t e = cudaMallocFromPoolAsync(out, bytes, dev->pool, s);
   if (e != cudaSuccess) {
     cudaGetLastError();
+    // An allocation that fails has taken what the device had left into the pool,
+    // which keeps what it has: give back all that is not in use.
+    cudaMemPoolTrimTo(dev->pool, 0);
+    cudaGetLastError();
     return fail(AGPU_ERR_OOM, "device pool: cannot allocate %zu bytes (%s)", bytes,
                 cudaGetErrorString(e));
   }

@@ -152,3 +152,20 @@ def test_signal_then_wait_flags_round_trip(dev):
     assert flags.cpu().tolist() == [0, 0, 0, 0]
     assert lib.agpu_wait_flags(dev.handle, C.c_void_p(flags.data_ptr()), 33, 1, 10, None) == 2
     assert lib.agpu_signal_peers(dev.handle, slots, 17, 1, None) == 2
+
+
+def test_allocation_that_fails_leaves_the_memory_to_others(dev):
+    """A buffer, and an op's scratch, that no device has room for (240 and 275 GB): what
+    the device had free is free again, for other pools and processes."""
+    import torch
+    from any_gpu import AnyGpuError, muon_tensors
+    torch.cuda.synchronize()
+    held = dev.upload(np.arange(1000))
+    before = torch.cuda.mem_get_info()[0]
+    far = muon_tensors([(1 << 52, 1 << 53, 1 << 54, 2**17, 2**17)])  # not memory: never read
+    for call in (lambda: dev.alloc(60 << 30), lambda: dev.launch_muon(far, 0.02)):
+        with pytest.raises(AnyGpuError) as e:
+            call()
+        assert e.value.status == 4
+        assert torch.cuda.mem_get_info()[0] >= before - (64 << 20)
+    np.testing.assert_array_equal(dev.read(held), np.arange(1000))

@@ -630,6 +630,7 @@ AGPU_API agpu_status agpu_launch_swish_mul(agpu_device* dev, const float* gate, 
                                            uint64_t out_stride, void* stream);
 AGPU_API agpu_status agpu_launch_softmax(agpu_device* dev, const float* x, float* y,
                                          uint64_t rows, uint32_t cols, void* stream);
+/* `out` must not overlap the table or the ids, nor `d_table` grad_out or the ids. */
 AGPU_API agpu_status agpu_launch_embedding(agpu_device* dev, const float* table,
                                            const int32_t* ids, float* out, uint64_t tokens,
                                            uint32_t vocab, uint32_t dim, float scale,
@@ -641,13 +642,15 @@ AGPU_API agpu_status agpu_launch_embedding_backward(agpu_device* dev, const floa
                                                     uint64_t tokens, uint32_t vocab,
                                                     uint32_t dim, float scale, int accumulate,
                                                     void* stream);
-/* Outputs may be the inputs themselves where the layouts are equal. */
+/* Outputs may be the inputs themselves where the layouts are equal; no other
+ * element may be shared (by an input and an output, or two outputs). */
 AGPU_API agpu_status agpu_launch_qk_norm_rope(agpu_device* dev, const agpu_qk_norm_rope* shape,
                                               const float* q, const float* k,
                                               const float* q_weight, const float* k_weight,
                                               const int32_t* positions, float* q_out,
                                               float* k_out, void* stream);
-/* d_q_weight / d_k_weight may be NULL; pool scratch when they are not. */
+/* d_q_weight / d_k_weight may be NULL; pool scratch when they are not.  Outputs
+ * share no element with an input or each other. */
 AGPU_API agpu_status agpu_launch_qk_norm_rope_backward(
     agpu_device* dev, const agpu_qk_norm_rope* shape, const float* d_q_out, const float* d_k_out,
     const float* q, const float* k, const float* q_weight, const float* k_weight,

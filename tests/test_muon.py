@@ -402,6 +402,45 @@ def test_out_of_memory_steps_no_matrix(dev, shapes):
 
 
 @gpu
+def test_batches_of_a_call_share_scratch(dev):
+    """Small ones on chip, two batches in steps on the Gram matrix (one of them of a single
+    matrix, columns dealt out) and two of the others, one after the other in the same
+    scratch: eager, and from a graph replayed for the second step."""
+    import torch
+    from any_gpu import muon_tensors
+    shapes = [(40, 70)] * 3 + [(512, 3000)] * 13 + [(300, 280)] * 25 + [(500, 40)]
+    r = np.random.default_rng(6)
+    start = [[_gradient(r, *s) for s in shapes] for _ in range(3)]
+    results = []
+    for graphed in (False, True):
+        hold = [[torch.from_numpy(a).cuda() for a in b] for b in start]
+        tensors = muon_tensors([(p.data_ptr(), g.data_ptr(), m.data_ptr(), *p.shape)
+                                for p, g, m in zip(*hold)])
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        call = lambda: dev.launch_muon(tensors, 0.02, 0.9, True, 0.1, 5, stream.cuda_stream)
+        graph = torch.cuda.CUDAGraph()
+        if graphed:
+            with torch.cuda.graph(graph, stream=stream):
+                call()
+        for step in range(2):
+            with torch.cuda.stream(stream):
+                graph.replay() if graphed else call()
+            torch.cuda.synchronize()
+            if step == 0 and not graphed:
+                for i in (0, 3, 15, 16, 39, 40, 41):
+                    want, _, size = _step(start[0][i], start[1][i], start[2][i], 0.02, 0.9, True,
+                                          0.1, 5)
+                    bound = (4 * U * (np.linalg.norm(want) + size)
+                             + (SEGMENTS if 3 <= i < 16 else TOL) * size)
+                    assert np.linalg.norm(hold[0][i].cpu().numpy() - want) <= bound
+        results.append(hold)
+    for a, b in zip(*results):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+@gpu
 def test_precision_mode_does_not_matter(dev):
     x = dev.upload(_gradient(np.random.default_rng(0), 256, 384))
     want = dev.read(dev.orthogonalize(x, 1, 256, 384))
